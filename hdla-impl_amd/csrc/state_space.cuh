@@ -1,0 +1,277 @@
+// What the kernels of the selective state space scan share: how its operands lie, how a wave takes them, and the step sizes.
+//
+// Per channel d with S states, decays A [D, S] (as they enter the exponent) and per-token B, C [G, S] that D / G channels share:
+//     delta_t = softplus(dt_t + bias);   h_t = exp(delta_t A) h_{t-1} + delta_t x_t B_t;   y_t = (C_t . h_t + D x_t) silu(z_t)
+//
+// Lanes: LPC lanes of a wave hold the states of one channel, four each, and a wave has 64 / LPC channels and L tokens at a time.  The W waves
+// of a workgroup take consecutive pieces of L tokens.  Every wave scans its piece from zero, the pieces' decays and ends meet in LDS, where one thread
+// a state chains them, and the wave walks its piece once more from the state that enters it.  The exponentials are formed once, four
+// issue slots each where a multiplication takes one, and stay in registers for the second walk: that one costs two slots a state.
+#pragma once
+#include "hdla_common.cuh"
+#include "row_tile.cuh"
+#include "../../include/hdla_state_space.h"
+
+#include <algorithm>
+
+namespace hdla {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// floats from one channel to the next of a piece of L tokens in LDS: 16 bytes aligned, neighbours on other banks
+constexpr int ss_pitch(int L) { return L + 4; }
+constexpr int SS_TOK = 8;             // tokens of a wave at a time
+constexpr int SS_CKPT = 64;           // tokens between the states that a forward pass leaves for the backward pass
+
+// element (b, t, .) of an operand: base + b batch + t row
+struct Operand {
+    const void* p;
+    long long batch, row;
+};
+struct ScanArgs {
+    Operand x, dt, z, B, C;           // z.p may be null; B, C: + group
+    long long B_group, C_group;
+    const void *A, *D, *bias;         // D, bias may be null
+    int A_f32, D_f32, bias_f32;
+    const float* h0;                  // [N, D, S], may be null
+    float* ht;                        // [N, D, S], may be null
+    void* y;                          // [rows, D]
+    float* ckpt;                      // [slots][blocks][64][4], may be null
+    const int64_t* cu;
+    int T, N, DD, S, G, softplus;
+    int per_group, blocks;            // channel blocks of a group, of all of them
+    // backward
+    const void* dy;                   // [rows, D]
+    const float* dht;
+    void *dx, *ddt, *dz;              // [rows, D]
+    float *part_bc, *part_a, *part_d, *part_bias, *dh0;
+    long long rows;
+    int slots;                        // sequences at a time
+};
+
+// V elements of T as they come from memory; VEC: with loads of several, else (rows at any address) one by one
+template <typename T, int V, bool VEC> struct Raw;
+template <int V> struct Raw<bf16, V, true> {
+    static constexpr int NW = V < 2 ? 1 : V / 2;
+    uint32_t w[NW];
+    __device__ __forceinline__ void load(const bf16* p) {
+        if constexpr (V == 1) w[0] = p->x;
+        else if constexpr (V == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
+        else if constexpr (V == 4) { const u32x2 r = *reinterpret_cast<const u32x2*>(p); w[0] = r[0]; w[1] = r[1]; }
+        else { const u32x4 r = *reinterpret_cast<const u32x4*>(p); w[0] = r[0]; w[1] = r[1]; w[2] = r[2]; w[3] = r[3]; }
+    }
+    __device__ __forceinline__ void load(const bf16* p, int) { load(p); }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
+};
+template <int V> struct Raw<bf16, V, false> {
+    uint32_t w[V];
+    // (the first n)
+    __device__ __forceinline__ void load(const bf16* p, int n) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = i < n ? p[i].x : 0;
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(w[i] << 16); }
+};
+template <int V, bool VEC> struct Raw<float, V, VEC> {
+    float w[V];
+    __device__ __forceinline__ void load(const float* p, int n) {
+        if constexpr (VEC && V % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+                const f32x4 r = *reinterpret_cast<const f32x4*>(p + i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[i + j] = r[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[i] = i < n ? p[i] : 0.f;
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = 0.f;
+    }
+    __device__ __forceinline__ float operator[](int i) const { return w[i]; }
+};
+// the first n of V results, rounded to nearest
+template <typename T, int V, bool VEC> __device__ __forceinline__ void st_values(T* p, const float (&x)[V], int n) {
+    if constexpr (VEC && V % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) st_frag(p + i, to_frag<T>(f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]}));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) st_elem(p + i, x[i]);
+    }
+}
+
+__device__ __forceinline__ float ld_param(const void* p, int f32, long long i) {
+    return f32 ? static_cast<const float*>(p)[i] : ld_elem(static_cast<const bf16*>(p) + i);
+}
+// four states of a channel, the first `n` of which there are
+__device__ __forceinline__ f32x4 ld_states(const float* p, int n, bool whole) {
+    if (whole) return *reinterpret_cast<const f32x4*>(p);
+    f32x4 r = zero4();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < n) r[j] = p[j];
+    return r;
+}
+__device__ __forceinline__ void st_states(float* p, f32x4 x, int n, bool whole) {
+    if (whole) { *reinterpret_cast<f32x4*>(p) = x; return; }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < n) p[j] = x[j];
+}
+
+// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) <= 1, and log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3: the series of artanh up to s^15
+// leaves 2 s^17 / 17 <= 1e-9, also relative to the result.  No logarithm, whose hardware form loses what is small beside one.
+template <typename T> __device__ __forceinline__ float softplus(float v) {
+    const float e = exp_t<T>(-fabsf(v)), s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+    float r = 2.f / 15.f;
+    r = __builtin_fmaf(r, q, 2.f / 13.f);
+    r = __builtin_fmaf(r, q, 2.f / 11.f);
+    r = __builtin_fmaf(r, q, 2.f / 9.f);
+    r = __builtin_fmaf(r, q, 2.f / 7.f);
+    r = __builtin_fmaf(r, q, 2.f / 5.f);
+    r = __builtin_fmaf(r, q, 2.f / 3.f);
+    r = __builtin_fmaf(r, q, 2.f);
+    return fmaxf(v, 0.f) + s * r;
+}
+template <typename T, int N> __device__ __forceinline__ void sigmoid_each(const float (&x)[N], float (&s)[N]) {
+    float e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = exp_t<T>(-x[i]);
+    sigmoid_of_exp<N>(e, s);
+}
+
+constexpr float LN2 = 0.69314718055994530942f;
+
+// Consecutive blocks of channels share cache lines: they go to workgroups of one XCD (which take the workgroups in turns).
+__device__ __forceinline__ int xcd_share(int id, int total) {
+    const int xcd = id & 7, q = total >> 3, r = total & 7;
+    return xcd * q + min(xcd, r) + (id >> 3);
+}
+
+// Where a lane stands: as a scanner (channel c, states 4 q .. 4 q + 3) and as a carrier of operands and results (token tok of the piece, V channels from ch)
+template <int LPC, int TOKENS> struct ScanLane {
+    static constexpr int CHN = 64 / LPC, V = TOKENS > LPC ? TOKENS / LPC : 1;
+    int c, q, tok, ch, d0, d, dv, left, carried, group;
+    bool live;
+    __device__ __forceinline__ ScanLane(const ScanArgs& p, int block) {
+        const int l = lane_id(), size = p.DD / p.G;
+        group = block / p.per_group;
+        const int first = (block - group * p.per_group) * CHN;
+        d0 = group * size + first;
+        c = l / LPC;
+        q = l % LPC;
+        d = d0 + c;
+        live = first + c < size;
+        left = live ? min(max(p.S - 4 * q, 0), 4) : 0;           // states of this lane that there are
+        tok = l / (CHN / V);                                      // (LPC = 16, eight tokens: beyond them on half of the lanes)
+        ch = l % (CHN / V) * V;
+        dv = d0 + ch;
+        carried = min(max(size - first - ch, 0), V);             // channels of these V that there are
+    }
+};
+
+// B or C of a wave's piece, its tokens x 4 LPC states, as fp32 in LDS: [tok][quad]
+template <typename T, int LPC, int TOKENS, bool VEC> struct StatesOf {
+    static constexpr int PIECES = TOKENS * LPC < 64 ? 1 : TOKENS * LPC / 64;
+    Raw<T, 4, VEC> r[PIECES];
+    __device__ __forceinline__ void load(const T* base, long long row, int tokens, int S) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int at = i * 64 + lane_id(), t = at / LPC, s = at % LPC * 4;
+            r[i].clear();
+            if (t < tokens && s < S) r[i].load(base + t * row + s, S - s);
+        }
+    }
+    __device__ __forceinline__ void put(f32x4* lds) const {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int at = i * 64 + lane_id();
+            if (PIECES * 64 <= TOKENS * LPC || at < TOKENS * LPC) lds[at] = f32x4{r[i][0], r[i][1], r[i][2], r[i][3]};
+        }
+    }
+};
+
+// Tokens stay in their order: left to itself the scheduler asks for the operands of all of them at once, and spills.
+__device__ __forceinline__ void apart() { __builtin_amdgcn_sched_barrier(0); }
+
+// sums over the LPC lanes of a channel
+template <int LPC, int N> __device__ __forceinline__ void sum_channel(float (&x)[N]) { sum_lanes<N>(x, LPC); }
+
+// first slot of a sequence in the states that a forward pass leaves: packed sequences' counts are not known to the host, and these never overlap
+__device__ __forceinline__ long long ckpt_slot(const ScanArgs& p, int n, int64_t bos) {
+    return p.cu ? bos / SS_CKPT + n : (long long)n * ((p.T + SS_CKPT - 1) / SS_CKPT);
+}
+inline long long ckpt_slots(bool packed, long long T, long long N) {
+    return packed ? T / SS_CKPT + N + 1 : N * ((T + SS_CKPT - 1) / SS_CKPT);
+}
+
+// ---- host side: what both passes and the workspace sizes go by ---------------------------------------------------------
+inline int lanes_of(int S) { return S <= 8 ? 2 : S <= 16 ? 4 : S <= 32 ? 8 : 16; }
+
+// What both passes and the workspace sizes go by
+struct ScanPlan {
+    int lpc, per_group, blocks, slots;
+    bool vec;
+    long long rows, ckpt;
+};
+inline bool fits(const void* p, int to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+inline int scan_plan(const hdla_scan_dims* d, ScanPlan& s) {
+    if (!d) return HDLA_ERR_NULL;
+    if (d->dtype != HDLA_BF16 && d->dtype != HDLA_FP32) return HDLA_ERR_DTYPE;
+    for (int t : {d->A_dtype, d->D_dtype, d->bias_dtype})
+        if (t != HDLA_BF16 && t != HDLA_FP32) return HDLA_ERR_DTYPE;
+    if (d->B < 1 || d->T < 0 || d->D < 1 || d->S < 1 || d->S > 64 || d->G < 1 || d->D % d->G || d->N < 1) return HDLA_ERR_SHAPE;
+    if (d->cu_seqlens ? d->B != 1 : d->N != d->B) return HDLA_ERR_SEQ;
+    if (d->T > (1 << 30) || d->D > (1 << 24)) return HDLA_ERR_SHAPE;
+    s.lpc = lanes_of(d->S);
+    const int channels = 64 / s.lpc, size = d->D / d->G;
+    s.per_group = (size + channels - 1) / channels;
+    s.blocks = d->G * s.per_group;
+    s.rows = (long long)d->B * d->T;
+    if ((long long)s.blocks * d->N > 0x7fffffffLL || s.rows > 0x7fffffffLL) return HDLA_ERR_SHAPE;
+    s.ckpt = ckpt_slots(d->cu_seqlens != nullptr, d->T, d->N);
+    s.slots = 1;
+    return HDLA_OK;
+}
+// Loads of V elements (channels) and of four (states): where everything lies on multiples of them
+inline bool scan_vec(const hdla_scan_dims* d, const ScanPlan& s, const ScanArgs& a) {
+    const int es = d->dtype == HDLA_BF16 ? 2 : 4, v = std::max(1, SS_TOK / s.lpc), size = d->D / d->G;
+    if (size % v || d->S % 4) return false;
+    const int bytes = std::min(v * es, 16);
+    for (const Operand* o : {&a.x, &a.dt, &a.z})
+        if (o->p && (!fits(o->p, bytes) || o->batch % v || o->row % v)) return false;
+    if (a.B_group % 4 || a.C_group % 4) return false;
+    for (const Operand* o : {&a.B, &a.C})
+        if (!fits(o->p, 4 * es) || o->batch % 4 || o->row % 4) return false;
+    return true;
+}
+
+inline ScanArgs scan_args(const hdla_scan_dims* d, const ScanPlan& s, const void* x, const void* dt, const void* A, const void* B, const void* C, const void* D,
+                          const void* z, const void* bias) {
+    ScanArgs a{};
+    a.x = {x, d->x_batch, d->x_row}; a.dt = {dt, d->dt_batch, d->dt_row}; a.z = {z, d->z_batch, d->z_row};
+    a.B = {B, d->B_batch, d->B_row}; a.C = {C, d->C_batch, d->C_row};
+    a.A = A; a.D = D; a.bias = bias;
+    a.B_group = d->B_group; a.C_group = d->C_group;
+    a.A_f32 = d->A_dtype == HDLA_FP32; a.D_f32 = d->D_dtype == HDLA_FP32; a.bias_f32 = d->bias_dtype == HDLA_FP32;
+    a.cu = d->cu_seqlens; a.T = d->T; a.N = d->N; a.DD = d->D; a.S = d->S; a.G = d->G; a.softplus = d->softplus != 0;
+    a.per_group = s.per_group; a.blocks = s.blocks; a.rows = s.rows; a.slots = s.slots;
+    return a;
+}
+
+}  // namespace hdla

@@ -1,0 +1,269 @@
+// The selective state space scan, forward (state_space.cuh has the formulas and how lanes and waves share the work), and its single-token step.
+//
+// What bounds the scan: the vector ALU.  A state and token cost one multiplication and one exponential (four issue slots) for the decay and six more
+// slots for the two walks, against 8 bytes of x, dt, z, y a channel and token of bf16.
+#include "state_space.cuh"
+#include "hdla_launch.h"
+
+namespace hdla {
+
+template <typename T, int LPC, int TOK, int W, bool VEC>
+__global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
+    using Lane = ScanLane<LPC, TOK>;
+    constexpr int CHN = Lane::CHN, V = Lane::V, TILE = W * TOK, PITCH = ss_pitch(TOK);
+    static_assert(W >= 4, "a thread a state of the 64 lanes");
+    __shared__ f32x4 sP[W][64], sE[W][64], sB[W][TOK * LPC], sC[W][TOK * LPC];
+    __shared__ __attribute__((aligned(16))) float sd[W][CHN * PITCH], sx[W][CHN * PITCH];
+
+    const int work = xcd_share(blockIdx.x, gridDim.x), n = work / p.blocks, block = work - n * p.blocks;
+    const int w = threadIdx.x >> 6, l = lane_id(), tid = threadIdx.x;
+    const Lane L(p, block);
+    int64_t bos = 0, eos = p.T;
+    if (p.cu) packed_bounds(p.cu, n, p.T, bos, eos);
+    const int len = (int)(eos - bos);
+    const bool whole = (p.S & 3) == 0;
+    const long long batch = p.cu ? 0 : n, row0 = p.cu ? bos : (long long)n * p.T;
+    auto start = [&](const Operand& o) { return static_cast<const T*>(o.p) + batch * o.batch + bos * o.row; };
+    const T *const x0 = start(p.x) + L.dv, *const dt0 = start(p.dt) + L.dv, *const z0 = p.z.p ? start(p.z) + L.dv : nullptr;
+    const T *const B0 = start(p.B) + L.group * p.B_group, *const C0 = start(p.C) + L.group * p.C_group;
+
+    f32x4 A2 = zero4();
+    float bias[V], D[V];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < L.left) A2[j] = ld_param(p.A, p.A_f32, (long long)L.d * p.S + 4 * L.q + j) * LOG2E;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        bias[i] = p.bias && i < L.carried ? ld_param(p.bias, p.bias_f32, L.dv + i) : 0.f;
+        D[i] = p.D && i < L.carried ? ld_param(p.D, p.D_f32, L.dv + i) : 0.f;
+    }
+    // The state that enters the tile, one of the 256 states of the block a thread of the first four waves: number tid of sE's rows
+    const int ec = (tid >> 2) / LPC, es = 4 * ((tid >> 2) % LPC) + (tid & 3);
+    const bool chains = tid < 256, there = chains && (block % p.per_group) * CHN + ec < p.DD / p.G && es < p.S;
+    const long long state = ((long long)n * p.DD + L.d0 + ec) * p.S + es;
+    float enters = there && p.h0 ? p.h0[state] : 0.f;
+
+    Raw<T, V, VEC> rx, rdt, rz;
+    StatesOf<T, LPC, TOK, VEC> rB, rC;
+    auto request = [&](int t0) __attribute__((always_inline)) {
+        const int tokens = min(max(len - t0, 0), TOK);
+        rx.clear(); rdt.clear(); rz.clear();
+        if (L.tok < tokens && L.carried > 0) {
+            const long long t = t0 + L.tok;
+            rx.load(x0 + t * p.x.row, L.carried);
+            rdt.load(dt0 + t * p.dt.row, L.carried);
+            if (z0) rz.load(z0 + t * p.z.row, L.carried);
+        }
+        rB.load(B0 + (long long)t0 * p.B.row, p.B.row, tokens, p.S);
+        rC.load(C0 + (long long)t0 * p.C.row, p.C.row, tokens, p.S);
+    };
+    request(w * TOK);
+    for (int tile = 0; tile < len; tile += TILE) {
+        const int t0 = tile + w * TOK, tokens = min(max(len - t0, 0), TOK);
+        float x[V], z[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            x[i] = rx[i];
+            z[i] = rz[i];
+            const float v = rdt[i] + bias[i], delta = L.tok < tokens ? (p.softplus ? softplus<T>(v) : v) : 0.f;
+            if (L.tok < TOK) {
+                sd[w][(L.ch + i) * PITCH + L.tok] = delta;
+                sx[w][(L.ch + i) * PITCH + L.tok] = delta * x[i];
+            }
+        }
+        rB.put(sB[w]);
+        rC.put(sC[w]);
+        request(t0 + TILE);
+        wave_lds_fence();
+        // from zero: the decays stay in registers
+        f32x4 a[TOK], E = zero4();
+        float u[TOK], sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < TOK; k += 4) {
+            const f32x4 dl = *reinterpret_cast<const f32x4*>(&sd[w][L.c * PITCH + k]), dx = *reinterpret_cast<const f32x4*>(&sx[w][L.c * PITCH + k]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 b = sB[w][(k + i) * LPC + L.q];
+                u[k + i] = dx[i];
+                sum += dl[i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    a[k + i][j] = __builtin_amdgcn_exp2f(dl[i] * A2[j]);
+                    E[j] = __builtin_fmaf(a[k + i][j], E[j], dx[i] * b[j]);
+                }
+                apart();
+            }
+        }
+        f32x4 P;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) P[j] = __builtin_amdgcn_exp2f(sum * A2[j]);
+        sP[w][l] = P;
+        sE[w][l] = E;
+        __syncthreads();
+        if (chains) {
+            float* const e = reinterpret_cast<float*>(sE) + tid;
+            const float* const f = reinterpret_cast<const float*>(sP) + tid;
+            float ends[W], decays[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) { ends[i] = e[i * 256]; decays[i] = f[i * 256]; }
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                e[i * 256] = enters;
+                enters = __builtin_fmaf(decays[i], enters, ends[i]);
+            }
+        }
+        __syncthreads();
+        f32x4 h = sE[w][l];
+        if (p.ckpt && t0 % SS_CKPT == 0 && tokens > 0)
+            *reinterpret_cast<f32x4*>(p.ckpt + (((ckpt_slot(p, n, bos) + t0 / SS_CKPT) * p.blocks + block) * 64 + l) * 4) = h;
+        float y[TOK];
+#pragma unroll
+        for (int k = 0; k < TOK; ++k) {
+            const f32x4 b = sB[w][k * LPC + L.q], cc = sC[w][k * LPC + L.q];
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                h[j] = __builtin_fmaf(a[k][j], h[j], u[k] * b[j]);
+                s = __builtin_fmaf(h[j], cc[j], s);
+            }
+            y[k] = s;
+            apart();
+        }
+        sum_channel<LPC>(y);
+        if (L.q == 0) {
+#pragma unroll
+            for (int k = 0; k < TOK; k += 4) *reinterpret_cast<f32x4*>(&sd[w][L.c * PITCH + k]) = f32x4{y[k], y[k + 1], y[k + 2], y[k + 3]};
+        }
+        wave_lds_fence();
+        float o[V], g[V];
+        if (z0) sigmoid_each<T, V>(z, g);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            o[i] = __builtin_fmaf(D[i], x[i], sd[w][(L.ch + i) * PITCH + min(L.tok, TOK - 1)]);
+            if (z0) o[i] *= z[i] * g[i];
+        }
+        if (L.tok < tokens && L.carried > 0)
+            st_values<T, V, VEC>(static_cast<T*>(p.y) + (row0 + t0 + L.tok) * p.DD + L.dv, o, L.carried);
+        wave_lds_fence();                                 // the next tile's operands go where y is
+    }
+    if (there && p.ht) p.ht[state] = enters;
+}
+
+// One token of each sequence: LPC lanes a channel, four states each.  Bound by HBM: 8 bytes a state.
+template <typename T>
+__global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs p, int lpc_log2) {
+    const int lpc = 1 << lpc_log2;
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x, channel = at >> lpc_log2;
+    const int q = (int)(at & (lpc - 1));
+    const bool live = channel < (long long)p.N * p.DD;
+    const long long ch = live ? channel : 0;
+    const int n = (int)(ch / p.DD), d = (int)(ch - (long long)n * p.DD), g = d / (p.DD / p.G), left = live ? min(max(p.S - 4 * q, 0), 4) : 0;
+    const bool whole = (p.S & 3) == 0 && left == 4;
+    auto elem = [&](const Operand& o, long long off) { return ld_elem(static_cast<const T*>(o.p) + n * o.batch + off); };
+    const long long so = ch * p.S + 4 * q;
+    f32x4 h = left ? ld_states(p.h0 + so, left, whole) : zero4(), A = zero4(), B = zero4(), C = zero4();
+    const float x = elem(p.x, d), v = elem(p.dt, d) + (p.bias ? ld_param(p.bias, p.bias_f32, d) : 0.f);
+    const float z = p.z.p ? elem(p.z, d) : 0.f;
+    const float D = p.D ? ld_param(p.D, p.D_f32, d) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (j < left) {
+            A[j] = ld_param(p.A, p.A_f32, (long long)d * p.S + 4 * q + j) * LOG2E;
+            B[j] = elem(p.B, g * p.B_group + 4 * q + j);
+            C[j] = elem(p.C, g * p.C_group + 4 * q + j);
+        }
+    }
+    const float delta = p.softplus ? softplus<T>(v) : v;
+    float y = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(delta * A[j]), h[j], delta * x * B[j]);
+        y = __builtin_fmaf(h[j], C[j], y);
+    }
+    y = sum_lanes(y, lpc);
+    if (left) st_states(p.ht + so, h, left, whole);
+    if (live && q == 0) {
+        y = __builtin_fmaf(D, x, y);
+        if (p.z.p) {
+            float zz[1] = {z}, s[1];
+            sigmoid_each<T, 1>(zz, s);
+            y *= z * s[0];
+        }
+        st_elem(static_cast<T*>(p.y) + ch, y);
+    }
+}
+
+template <typename T, int LPC, int L, int W> static void launch_tokens(const ScanArgs& a, bool vec, hipStream_t s) {
+    const dim3 grid((unsigned)((long long)a.blocks * a.N)), block(64 * W);
+    if (vec) hipLaunchKernelGGL((scan_tokens_kernel<T, LPC, L, W, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((scan_tokens_kernel<T, LPC, L, W, false>), grid, block, 0, s, a);
+}
+template <typename T> static hipError_t launch_scan(const ScanArgs& a, const ScanPlan& s, hipStream_t st) {
+    const int average = a.T / (a.cu ? a.N : 1);
+    const bool few = average <= 64;
+    switch (s.lpc) {
+#define HDLA_SCAN_CASE(LPCV)                                                          \
+    case LPCV:                                                                        \
+        if (few) launch_tokens<T, LPCV, SS_TOK, 4>(a, s.vec, st);                             \
+        else launch_tokens<T, LPCV, SS_TOK, 8>(a, s.vec, st);                                 \
+        break;
+        HDLA_SCAN_CASE(2)
+        HDLA_SCAN_CASE(4)
+        HDLA_SCAN_CASE(8)
+        HDLA_SCAN_CASE(16)
+#undef HDLA_SCAN_CASE
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace hdla
+
+using namespace hdla;
+
+extern "C" int hdla_state_space_version(void) { return HDLA_STATE_SPACE_VERSION; }
+extern "C" int hdla_scan_fwd(const hdla_scan_dims* dims, const void* x, const void* dt, const void* A, const void* B, const void* C, const void* D, const void* z,
+                             const void* dt_bias, const float* h0, void* y, float* ht, void* states, size_t states_bytes, void* stream) {
+    ScanPlan s;
+    const int rc = scan_plan(dims, s);
+    if (rc) return rc;
+    if (s.rows > 0 && (!x || !dt || !A || !B || !C || !y)) return HDLA_ERR_NULL;
+    if (!fits(y, 16) || !fits(h0, 16) || !fits(ht, 16)) return HDLA_ERR_ALIGN;
+    if (states && (!fits(states, 16) || states_bytes < (size_t)s.ckpt * s.blocks * 1024)) return HDLA_ERR_WORKSPACE;
+    ScanArgs a = scan_args(dims, s, x, dt, A, B, C, D, z, dt_bias);
+    a.h0 = h0; a.ht = ht; a.y = y; a.ckpt = static_cast<float*>(states);
+    s.vec = scan_vec(dims, s, a);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (a.cu) {
+        PackedOut out{};
+        out.add(y, (long long)dims->D * (dims->dtype == HDLA_BF16 ? 2 : 4));
+        const hipError_t e = launch_clear_uncovered(a.cu, a.N, a.T, out, st);
+        if (e != hipSuccess) return (int)e;
+    }
+    const hipError_t e = dims->dtype == HDLA_BF16 ? launch_scan<bf16>(a, s, st) : launch_scan<float>(a, s, st);
+    return e == hipSuccess ? HDLA_OK : (int)e;
+}
+extern "C" size_t hdla_scan_states_bytes(const hdla_scan_dims* dims) {
+    ScanPlan s;
+    return scan_plan(dims, s) ? 0 : (size_t)s.ckpt * s.blocks * 1024;
+}
+extern "C" int hdla_scan_step(const hdla_scan_dims* dims, const void* x, const void* dt, const void* A, const void* B, const void* C, const void* D, const void* z,
+                              const void* dt_bias, const float* state, void* y, float* new_state, void* stream) {
+    ScanPlan s;
+    const int rc = scan_plan(dims, s);
+    if (rc) return rc;
+    if (dims->T != 1 || dims->cu_seqlens) return HDLA_ERR_SHAPE;
+    if (!x || !dt || !A || !B || !C || !y || !state || !new_state) return HDLA_ERR_NULL;
+    if (!fits(y, 16) || !fits(state, 16) || !fits(new_state, 16)) return HDLA_ERR_ALIGN;
+    ScanArgs a = scan_args(dims, s, x, dt, A, B, C, D, z, dt_bias);
+    a.h0 = state; a.ht = new_state; a.y = y;
+    int log2 = 0;
+    while ((4 << log2) < dims->S) ++log2;
+    const long long threads = (long long)a.N * a.DD << log2, blocks = (threads + 255) / 256;
+    if (blocks > 0x7fffffffLL) return HDLA_ERR_SHAPE;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dims->dtype == HDLA_BF16) hipLaunchKernelGGL(scan_step_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, st, a, log2);
+    else hipLaunchKernelGGL(scan_step_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, a, log2);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? HDLA_OK : (int)e;
+}

@@ -1,0 +1,362 @@
+// The selective state space scan's backward pass.  With e_t = dy_t silu(z_t) and G_t the gradient of h_t,
+//     G_t = C_t e_t + exp(delta_{t+1} A) G_{t+1};   u_t = exp(delta_t A) h_{t-1};
+//     dC_t = sum_d e h;  dB_t = sum_d G delta x;  dx = delta sum_s G B + D e;  d delta = sum_s G (A u + x B);  dA = sum_t G delta u;
+//     dD = sum_t e x;  dz = dy (C . h + D x) silu'(z);  dh_0 = exp(delta_1 A) G_1.
+// Tiles of 64 tokens, the last first, each from the state that the forward pass left at its first token.  A wave scans its eight tokens forwards and backwards
+// from zero; both chains over the waves' pieces run at once, four waves each; then it walks them again with what enters, states and decays in registers.
+//
+// What bounds it: the vector ALU, some 26 issue slots a state and token, of which four are the exponential and four the sums over channels for dB and dC.
+#include "column_sums.cuh"
+#include "hdla_launch.h"
+#include "state_space.cuh"
+
+namespace hdla {
+
+// x and y of all lanes: their sums over pairs of lanes that are 32 (16) apart, x's in the lower half (the even rows of 16), y's in the upper (odd ones)
+__device__ __forceinline__ float fold32(float x, float y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(y), false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+__device__ __forceinline__ float fold16(float x, float y) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(y), false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+
+template <typename T, int LPC, int TOK, int W, bool VEC>
+__global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
+    using Lane = ScanLane<LPC, TOK>;
+    constexpr int CHN = Lane::CHN, V = Lane::V, TILE = W * TOK, PITCH = ss_pitch(TOK);
+    static_assert(W >= 8 && TILE % SS_CKPT == 0, "a thread a state for either chain; a tile begins where a state is left");
+    __shared__ f32x4 sP[W][64], sE[W][64], sG[W][64], sB[W][TOK * LPC], sC[W][TOK * LPC];
+    __shared__ __attribute__((aligned(16))) float sd[W][CHN * PITCH], sx[W][CHN * PITCH], se[W][CHN * PITCH], sy[W][CHN * PITCH];
+
+    const int work = xcd_share(blockIdx.x, gridDim.x), slot = work / p.blocks, block = work - slot * p.blocks;
+    const int w = threadIdx.x >> 6, l = lane_id(), tid = threadIdx.x;
+    const Lane L(p, block);
+    f32x4 A2 = zero4(), dA = zero4();
+    float bias[V], D[V], dD[V], dbias[V];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < L.left) A2[j] = ld_param(p.A, p.A_f32, (long long)L.d * p.S + 4 * L.q + j) * LOG2E;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        bias[i] = p.bias && i < L.carried ? ld_param(p.bias, p.bias_f32, L.dv + i) : 0.f;
+        D[i] = p.D && i < L.carried ? ld_param(p.D, p.D_f32, L.dv + i) : 0.f;
+        dD[i] = dbias[i] = 0.f;
+    }
+    // a thread a state: the first four waves chain the states, the other four their gradients
+    const int e = tid & 255, ec = (e >> 2) / LPC, es = 4 * ((e >> 2) % LPC) + (e & 3);
+    const bool forwards = tid < 256, backwards = tid >= 256 && tid < 512, there = (block % p.per_group) * CHN + ec < p.DD / p.G && es < p.S;
+
+    for (int n = slot; n < p.N; n += p.slots) {
+        int64_t bos = 0, eos = p.T;
+        if (p.cu) packed_bounds(p.cu, n, p.T, bos, eos);
+        const int len = (int)(eos - bos);
+        const long long batch = p.cu ? 0 : n, row0 = p.cu ? bos : (long long)n * p.T;
+        auto start = [&](const Operand& o) { return static_cast<const T*>(o.p) + batch * o.batch + bos * o.row; };
+        const T *const x0 = start(p.x) + L.dv, *const dt0 = start(p.dt) + L.dv, *const z0 = p.z.p ? start(p.z) + L.dv : nullptr;
+        const T *const B0 = start(p.B) + L.group * p.B_group, *const C0 = start(p.C) + L.group * p.C_group;
+        const T* const dy0 = static_cast<const T*>(p.dy) + row0 * p.DD + L.dv;
+        const long long state = ((long long)n * p.DD + L.d0 + ec) * p.S + es;
+        float enters = backwards && there && p.dht ? p.dht[state] : 0.f;
+
+        Raw<T, V, VEC> rx, rdt, rz, rdy;
+        StatesOf<T, LPC, TOK, VEC> rB, rC;
+        auto request = [&](int t0) __attribute__((always_inline)) {
+            const int tokens = t0 < 0 ? 0 : min(max(len - t0, 0), TOK);
+            rx.clear(); rdt.clear(); rz.clear(); rdy.clear();
+            if (L.tok < tokens && L.carried > 0) {
+                const long long t = t0 + L.tok;
+                rx.load(x0 + t * p.x.row, L.carried);
+                rdt.load(dt0 + t * p.dt.row, L.carried);
+                if (z0) rz.load(z0 + t * p.z.row, L.carried);
+                rdy.load(dy0 + t * p.DD, L.carried);
+            }
+            rB.load(B0 + (long long)t0 * p.B.row, p.B.row, tokens, p.S);
+            rC.load(C0 + (long long)t0 * p.C.row, p.C.row, tokens, p.S);
+        };
+        const int tiles = (len + TILE - 1) / TILE;
+        request((tiles - 1) * TILE + w * TOK);
+        for (int tile = tiles - 1; tile >= 0; --tile) {
+            const int t0 = tile * TILE + w * TOK, tokens = min(max(len - t0, 0), TOK);
+            const float left = forwards ? p.ckpt[((ckpt_slot(p, n, bos) + tile * (TILE / SS_CKPT)) * p.blocks + block) * 256 + e] : 0.f;
+            float x[V], z[V], dy[V], v[V], gz[V], delta[V], ee[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) { x[i] = rx[i]; z[i] = rz[i]; dy[i] = rdy[i]; v[i] = rdt[i] + bias[i]; }
+            if (z0) sigmoid_each<T, V>(z, gz);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                delta[i] = L.tok < tokens ? (p.softplus ? softplus<T>(v[i]) : v[i]) : 0.f;
+                ee[i] = z0 ? dy[i] * (z[i] * gz[i]) : dy[i];
+                const int at = (L.ch + i) * PITCH + L.tok;
+                if (L.tok < TOK) {
+                    sd[w][at] = delta[i];
+                    sx[w][at] = delta[i] * x[i];
+                    se[w][at] = ee[i];
+                }
+            }
+            rB.put(sB[w]);
+            rC.put(sC[w]);
+            request(t0 - TILE);
+            wave_lds_fence();
+            f32x4 a[TOK], E = zero4(), G = zero4();
+            const float *const mine_d = &sd[w][L.c * PITCH], *const mine_x = &sx[w][L.c * PITCH], *const mine_e = &se[w][L.c * PITCH];
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < TOK; ++k) {
+                const f32x4 b = sB[w][k * LPC + L.q];
+                const float dl = mine_d[k], u = mine_x[k];
+                sum += dl;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    a[k][j] = __builtin_amdgcn_exp2f(dl * A2[j]);
+                    E[j] = __builtin_fmaf(a[k][j], E[j], u * b[j]);
+                }
+                apart();
+            }
+#pragma unroll
+            for (int k = TOK - 1; k >= 0; --k) {
+                const f32x4 cc = sC[w][k * LPC + L.q];
+                const float ev = mine_e[k];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) G[j] = a[k][j] * __builtin_fmaf(cc[j], ev, G[j]);
+                apart();
+            }
+            f32x4 P;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) P[j] = __builtin_amdgcn_exp2f(sum * A2[j]);
+            sP[w][l] = P;
+            sE[w][l] = E;
+            sG[w][l] = G;
+            __syncthreads();
+            if (tid < 512) {
+                float* const at = reinterpret_cast<float*>(forwards ? sE : sG) + e;
+                const float* const f = reinterpret_cast<const float*>(sP) + e;
+                float ends[W], decays[W];
+#pragma unroll
+                for (int i = 0; i < W; ++i) { ends[i] = at[i * 256]; decays[i] = f[i * 256]; }
+                if (forwards) {
+                    enters = left;
+#pragma unroll
+                    for (int i = 0; i < W; ++i) {
+                        at[i * 256] = enters;
+                        enters = __builtin_fmaf(decays[i], enters, ends[i]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = W - 1; i >= 0; --i) {
+                        at[i * 256] = enters;
+                        enters = __builtin_fmaf(decays[i], enters, ends[i]);
+                    }
+                }
+            }
+            __syncthreads();
+            const f32x4 first = sE[w][l];
+            G = sG[w][l];
+            f32x4 h[TOK];
+#pragma unroll
+            for (int k = 0; k < TOK; ++k) {
+                const f32x4 b = sB[w][k * LPC + L.q], cc = sC[w][k * LPC + L.q];
+                const float u = mine_x[k];
+                float y[1] = {0.f};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    h[k][j] = __builtin_fmaf(a[k][j], k ? h[k - 1][j] : first[j], u * b[j]);
+                    y[0] = __builtin_fmaf(h[k][j], cc[j], y[0]);
+                }
+                sum_channel<LPC>(y);
+                sy[w][L.c * PITCH + k] = y[0];            // (the same from all lanes of the channel)
+                apart();
+            }
+            wave_lds_fence();                             // B and C are read again, not kept
+#pragma unroll
+            for (int k = TOK - 1; k >= 0; --k) {
+                const f32x4 b = sB[w][k * LPC + L.q], cc = sC[w][k * LPC + L.q];
+                const float dl = mine_d[k], u = mine_x[k], ev = mine_e[k];
+                float s[2] = {0.f, 0.f}, db[4], dc[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float g = __builtin_fmaf(cc[j], ev, G[j]);
+                    dc[j] = ev * h[k][j];
+                    db[j] = g * u;
+                    s[0] = __builtin_fmaf(g, b[j], s[0]);
+                    G[j] = a[k][j] * g;
+                    const float through = G[j] * (k ? h[k - 1][j] : first[j]);
+                    s[1] = __builtin_fmaf(through, A2[j], s[1]);
+                    dA[j] = __builtin_fmaf(through, dl, dA[j]);
+                }
+                // over the wave's channels: lanes with the same states
+                float f0 = fold16(fold32(db[0], dc[0]), fold32(db[1], dc[1])), f1 = fold16(fold32(db[2], dc[2]), fold32(db[3], dc[3]));
+                if constexpr (LPC < 16) { f0 += dpp0<0x128>(f0); f1 += dpp0<0x128>(f1); }      // row_ror:8
+                if constexpr (LPC < 8) { f0 += dpp0<0x124>(f0); f1 += dpp0<0x124>(f1); }
+                if constexpr (LPC < 4) { f0 += dpp0<0x122>(f0); f1 += dpp0<0x122>(f1); }
+                sum_channel<LPC>(s);
+                // (what this token had there has been read: B, C, delta, delta x)
+                sd[w][L.c * PITCH + k] = s[0];
+                sx[w][L.c * PITCH + k] = s[1];
+                if ((l & 15) < LPC) {
+                    float* const to = reinterpret_cast<float*>(&(l < 32 ? sB : sC)[w][k * LPC + (l & 15)]) + ((l >> 4) & 1);
+                    to[0] = f0;
+                    to[2] = f1;
+                }
+                apart();
+            }
+            wave_lds_fence();
+            float ox[V], odt[V], oz[V], sv[V];
+            if (p.softplus) sigmoid_each<T, V>(v, sv);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int at = (L.ch + i) * PITCH + min(L.tok, TOK - 1);
+                const float gb = sd[w][at], ga = sx[w][at] * LN2, inner = __builtin_fmaf(D[i], x[i], sy[w][at]);
+                ox[i] = __builtin_fmaf(D[i], ee[i], gb * delta[i]);
+                odt[i] = __builtin_fmaf(gb, x[i], ga);
+                if (p.softplus) odt[i] *= sv[i];
+                if (z0) oz[i] = dy[i] * inner * (gz[i] * __builtin_fmaf(z[i], 1.f - gz[i], 1.f));
+                if (L.tok < tokens) {
+                    dD[i] = __builtin_fmaf(ee[i], x[i], dD[i]);
+                    dbias[i] += odt[i];
+                }
+            }
+            if (L.tok < tokens && L.carried > 0) {
+                const long long at = (row0 + t0 + L.tok) * p.DD + L.dv;
+                st_values<T, V, VEC>(static_cast<T*>(p.dx) + at, ox, L.carried);
+                st_values<T, V, VEC>(static_cast<T*>(p.ddt) + at, odt, L.carried);
+                if (z0) st_values<T, V, VEC>(static_cast<T*>(p.dz) + at, oz, L.carried);
+            }
+            // this block's part of dB and dC: [block of the group][B, C][row][group][S]
+            {
+                const long long inner = (long long)p.G * p.S, half = p.rows * inner;
+                float* const to = p.part_bc + 2 * half * (block % p.per_group) + (row0 + t0) * inner + (long long)L.group * p.S;
+                constexpr int PIECES = TOK * LPC < 64 ? 1 : TOK * LPC / 64;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) {
+                    const int at = i * 64 + l, t = at / LPC, s = at % LPC * 4;
+                    if (t < tokens && s < p.S) {
+                        st_states(to + t * inner + s, sB[w][at], p.S - s, VEC);
+                        st_states(to + half + t * inner + s, sC[w][at], p.S - s, VEC);
+                    }
+                }
+            }
+            wave_lds_fence();
+        }
+        if (backwards && there && p.dh0) p.dh0[state] = enters;
+    }
+    // what the waves have of dA, dD and d bias
+    __syncthreads();
+    sE[w][l] = dA;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        // over the tokens
+#pragma unroll
+        for (int m = CHN / V; m < 64; m *= 2) { dD[i] += __shfl_xor(dD[i], m); dbias[i] += __shfl_xor(dbias[i], m); }
+        if (l < CHN / V) { sd[w][L.ch + i] = dD[i]; sx[w][L.ch + i] = dbias[i]; }
+    }
+    __syncthreads();
+    if (tid < 256) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) s += reinterpret_cast<const float*>(sE)[i * 256 + e];
+        if (there) p.part_a[((long long)slot * p.DD + L.d0 + ec) * p.S + es] = s;
+    } else if (backwards && e < CHN && (block % p.per_group) * CHN + e < p.DD / p.G) {
+        float s = 0.f, b = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) { s += sd[i][e]; b += sx[i][e]; }
+        p.part_d[(long long)slot * p.DD + L.d0 + e] = s;
+        p.part_bias[(long long)slot * p.DD + L.d0 + e] = b;
+    }
+}
+
+// Workgroups walk sequences in turns so that their partial sums of dA, dD and d bias stay few: as many as fill the device a few times
+static int grad_slots(const hdla_scan_dims* d, const ScanPlan& s) {
+    const long long most = std::max(1LL, 2048LL / s.blocks);
+    return (int)std::min<long long>(d->N, most);
+}
+struct GradRoom { size_t bc, a, d, bias, total; };
+static GradRoom grad_room(const hdla_scan_dims* d, const ScanPlan& s, int slots) {
+    auto up = [](size_t n) { return (n + 15) / 16 * 16; };
+    GradRoom r;
+    r.bc = 0;
+    r.a = up((size_t)s.per_group * 2 * s.rows * d->G * d->S * 4);
+    r.d = r.a + up((size_t)slots * d->D * d->S * 4);
+    r.bias = r.d + up((size_t)slots * d->D * 4);
+    r.total = r.bias + up((size_t)slots * d->D * 4);
+    return r;
+}
+template <typename T, int LPC> static void launch_grad(const ScanArgs& a, bool vec, hipStream_t s) {
+    constexpr int TOK = SS_TOK, W = 8;
+    const dim3 grid((unsigned)((long long)a.blocks * a.slots)), block(64 * W);
+    if (vec) hipLaunchKernelGGL((scan_grad_kernel<T, LPC, TOK, W, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((scan_grad_kernel<T, LPC, TOK, W, false>), grid, block, 0, s, a);
+}
+template <typename T> static hipError_t launch_scan_grad(const ScanArgs& a, const ScanPlan& s, hipStream_t st) {
+    switch (s.lpc) {
+        case 2: launch_grad<T, 2>(a, s.vec, st); break;
+        case 4: launch_grad<T, 4>(a, s.vec, st); break;
+        case 8: launch_grad<T, 8>(a, s.vec, st); break;
+        case 16: launch_grad<T, 16>(a, s.vec, st); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace hdla
+
+using namespace hdla;
+
+extern "C" size_t hdla_scan_workspace_bytes(const hdla_scan_dims* dims) {
+    ScanPlan s;
+    return scan_plan(dims, s) ? 0 : grad_room(dims, s, grad_slots(dims, s)).total;
+}
+extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const void* dt, const void* A, const void* B, const void* C, const void* D, const void* z,
+                             const void* dt_bias, const void* dy, const float* dht, const void* states, size_t states_bytes, void* dx, void* ddt, void* dA, void* dB,
+                             void* dC, void* dD, void* dz, void* ddt_bias, float* dh0, void* workspace, size_t workspace_bytes, void* stream) {
+    ScanPlan s;
+    const int rc = scan_plan(dims, s);
+    if (rc) return rc;
+    if (!A || !dA || (D && !dD) || (dt_bias && !ddt_bias)) return HDLA_ERR_NULL;
+    if (s.rows > 0 && (!x || !dt || !B || !C || !dy || !dx || !ddt || !dB || !dC || !states || (z && !dz))) return HDLA_ERR_NULL;
+    for (const void* q : {dy, (const void*)dht, states, (const void*)dx, (const void*)ddt, (const void*)dB, (const void*)dC, (const void*)dz, (const void*)dh0})
+        if (!fits(q, 16)) return HDLA_ERR_ALIGN;
+    s.slots = grad_slots(dims, s);
+    const GradRoom room = grad_room(dims, s, s.slots);
+    if (!workspace || !fits(workspace, 16) || workspace_bytes < room.total) return HDLA_ERR_WORKSPACE;
+    if (s.rows > 0 && states_bytes < (size_t)s.ckpt * s.blocks * 1024) return HDLA_ERR_WORKSPACE;
+    ScanArgs a = scan_args(dims, s, x, dt, A, B, C, D, z, dt_bias);
+    a.dy = dy; a.dht = dht; a.ckpt = static_cast<float*>(const_cast<void*>(states));
+    a.dx = dx; a.ddt = ddt; a.dz = dz; a.dh0 = dh0;
+    char* const base = static_cast<char*>(workspace);
+    a.part_bc = reinterpret_cast<float*>(base + room.bc);
+    a.part_a = reinterpret_cast<float*>(base + room.a);
+    a.part_d = reinterpret_cast<float*>(base + room.d);
+    a.part_bias = reinterpret_cast<float*>(base + room.bias);
+    s.vec = scan_vec(dims, s, a);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const int es = dims->dtype == HDLA_BF16 ? 2 : 4;
+    if (a.cu) {
+        PackedOut out{};
+        for (void* o : {dx, ddt, dz}) out.add(o, (long long)dims->D * es);
+        const hipError_t e = launch_clear_uncovered(a.cu, a.N, a.T, out, st);
+        if (e != hipSuccess) return (int)e;
+    }
+    hipError_t e = dims->dtype == HDLA_BF16 ? launch_scan_grad<bf16>(a, s, st) : launch_scan_grad<float>(a, s, st);
+    if (e != hipSuccess) return (int)e;
+    ColumnSums c{};
+    const long long inner = (long long)dims->G * dims->S;
+    c.part = a.part_bc; c.rows = s.per_group;
+    c.cu = a.cu; c.N = a.N; c.T = a.T; c.per_token = inner; c.tokens_end = 2 * s.rows * inner;
+    c.add(dB, es == 4, s.rows * inner);
+    c.add(dC, es == 4, s.rows * inner);
+    e = launch_column_sums(c, st);
+    if (e != hipSuccess) return (int)e;
+    const struct { const float* part; void* out; int f32; long long n; } sums[3] = {
+        {a.part_a, dA, a.A_f32, (long long)dims->D * dims->S}, {a.part_d, dD, a.D_f32, dims->D}, {a.part_bias, ddt_bias, a.bias_f32, dims->D}};
+    for (const auto& q : sums) {
+        if (!q.out) continue;
+        ColumnSums k{};
+        k.part = q.part; k.rows = s.slots;
+        k.add(q.out, q.f32, q.n);
+        e = launch_column_sums(k, st);
+        if (e != hipSuccess) return (int)e;
+    }
+    return HDLA_OK;
+}

@@ -1,4 +1,4 @@
-"""ctypes binding of libhdla_hip.so (the C ABI declared in include/hdla_hip.h).
+"""ctypes binding of libhdla_hip.so (the C ABI declared in include/hdla_hip.h and include/hdla_state_space.h).
 
 The library is the only compute path: if it cannot be loaded every operator raises, there is no fallback.
 """
@@ -13,6 +13,7 @@ import torch
 
 HDLA_BF16, HDLA_FP32 = 0, 1
 HDLA_VERSION = 211          # the header this binding was written against (struct layouts, entry points)
+STATE_SPACE_VERSION = 1      # the same of include/hdla_state_space.h
 ROUTE_AUTO, ROUTE_CLASSIC, ROUTE_FUSED, ROUTE_PLAIN = 0, 1, 2, 4
 _ROUTES = {"": ROUTE_AUTO, "auto": ROUTE_AUTO, "classic": ROUTE_CLASSIC, "plain": ROUTE_PLAIN, "fused": ROUTE_FUSED}
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -56,6 +57,25 @@ class HdlaUpDims(ctypes.Structure):
                 ("col_f", ctypes.c_int32), ("col_g", ctypes.c_int32)]
 
 
+class HdlaConvDims(ctypes.Structure):
+    """struct hdla_conv_dims of include/hdla_state_space.h."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "T", "D", "W", "N", "dtype", "weight_dtype", "bias_dtype", "silu")] + [
+        ("x_batch", ctypes.c_int64), ("x_row", ctypes.c_int64), ("cu_seqlens", ctypes.c_void_p)]
+
+
+class HdlaScanDims(ctypes.Structure):
+    """struct hdla_scan_dims of include/hdla_state_space.h."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "T", "D", "S", "G", "N", "dtype", "A_dtype", "D_dtype", "bias_dtype", "softplus")] + [
+        (n, ctypes.c_int64) for n in ("x_batch", "x_row", "dt_batch", "dt_row", "z_batch", "z_row", "B_batch", "B_row", "B_group", "C_batch", "C_row",
+                                      "C_group")] + [("cu_seqlens", ctypes.c_void_p)]
+
+
+class HdlaBlockNormDims(ctypes.Structure):
+    """struct hdla_block_norm_dims of include/hdla_state_space.h."""
+    _fields_ = [("rows", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in (
+        "E", "dtype", "residual_dtype", "weight_dtype", "post_dtype", "scale_dtype", "act", "post_norm")] + [("factor", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
 class HdlaError(RuntimeError):
     pass
 
@@ -81,6 +101,8 @@ def load():
     if lib.hdla_version() != HDLA_VERSION:
         raise HdlaError(f"{path} is version {lib.hdla_version()} of the C ABI, this binding needs {HDLA_VERSION}: "
                         "rebuild the library (make -C hdla-impl_amd/csrc)")
+    if not hasattr(lib, "hdla_state_space_version") or lib.hdla_state_space_version() != STATE_SPACE_VERSION:
+        raise HdlaError(f"{path} has not the state space operators of version {STATE_SPACE_VERSION}: rebuild the library (make -C hdla-impl_amd/csrc)")
     lib.hdla_strerror.restype = ctypes.c_char_p
     lib.hdla_strerror.argtypes = [ctypes.c_int]
     lib.hdla_workspace_bytes.restype = ctypes.c_size_t
@@ -169,6 +191,16 @@ def load():
     lib.hdla_weight_grad_pair_workspace_bytes.argtypes = [ctypes.c_int64, P, P]
     lib.hdla_weight_grad_pair.restype = ctypes.c_int
     lib.hdla_weight_grad_pair.argtypes = [ctypes.c_int64, P, P, P, P, P, P, P, P, ctypes.c_size_t, P, P]
+    CF, SF, BF, Z = ctypes.POINTER(HdlaConvDims), ctypes.POINTER(HdlaScanDims), ctypes.POINTER(HdlaBlockNormDims), ctypes.c_size_t
+    for name, result, arguments in (
+            ("short_conv_fwd", ctypes.c_int, [CF] + [P] * 7), ("short_conv_workspace_bytes", Z, [CF]), ("short_conv_bwd", ctypes.c_int, [CF] + [P] * 11 + [Z, P]),
+            ("short_conv_step", ctypes.c_int, [CF] + [P] * 7),
+            ("scan_states_bytes", Z, [SF]), ("scan_fwd", ctypes.c_int, [SF] + [P] * 12 + [Z, P]), ("scan_workspace_bytes", Z, [SF]),
+            ("scan_bwd", ctypes.c_int, [SF] + [P] * 11 + [Z] + [P] * 10 + [Z, P]), ("scan_step", ctypes.c_int, [SF] + [P] * 12),
+            ("block_norm_fwd", ctypes.c_int, [BF] + [P] * 9), ("block_norm_workspace_bytes", Z, [BF]),
+            ("block_norm_bwd", ctypes.c_int, [BF] + [P] * 15 + [Z, P])):
+        fn = getattr(lib, "hdla_" + name)
+        fn.restype, fn.argtypes = result, arguments
     lib.hdla_stack_rows.restype = ctypes.c_int
     lib.hdla_stack_rows.argtypes = [P, P, ctypes.c_int32, ctypes.c_int64, P, ctypes.c_int64, P]
     _lib = lib
