@@ -21,14 +21,18 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // floats from one channel to the next of a piece of L tokens in LDS: 16 bytes aligned, neighbours on other banks
 constexpr int ss_pitch(int L) { return L + 4; }
-constexpr int SS_TOK = 8;             // tokens of a wave at a time
+constexpr int SS_TOK = 8;             // tokens of a wave at a time; the forward pass takes twice as many of long sequences (not of 32 channels a wave: registers)
 constexpr int SS_CKPT = 64;           // tokens between the states that a forward pass leaves for the backward pass
 
-// element (b, t, .) of an operand: base + b batch + t row
+// element (b, t, .) of an operand: base + b batch + t row.  A wave's tokens are reached by 32-bit offsets from its first one's row.
 struct Operand {
     const void* p;
     long long batch, row;
 };
+constexpr long long ROW_MOST = 1 << 24;      // elements; 16 rows of 4 bytes reach 2^30
+template <typename T> __device__ __forceinline__ const T* row_of(const Operand& o, long long batch, long long t) {
+    return static_cast<const T*>(o.p) + batch * o.batch + t * o.row;
+}
 struct ScanArgs {
     Operand x, dt, z, B, C;           // z.p may be null; B, C: + group
     long long B_group, C_group;
@@ -55,25 +59,35 @@ template <typename T, int V, bool VEC> struct Raw;
 template <int V> struct Raw<bf16, V, true> {
     static constexpr int NW = V < 2 ? 1 : V / 2;
     uint32_t w[NW];
-    __device__ __forceinline__ void load(const bf16* p) {
+    __device__ __forceinline__ void load(const bf16* p, int) {
         if constexpr (V == 1) w[0] = p->x;
         else if constexpr (V == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
         else if constexpr (V == 4) { const u32x2 r = *reinterpret_cast<const u32x2*>(p); w[0] = r[0]; w[1] = r[1]; }
         else { const u32x4 r = *reinterpret_cast<const u32x4*>(p); w[0] = r[0]; w[1] = r[1]; w[2] = r[2]; w[3] = r[3]; }
     }
-    __device__ __forceinline__ void load(const bf16* p, int) { load(p); }
+    template <typename R> __device__ __forceinline__ void load(R rows, uint32_t off, int) {
+        if constexpr (V == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b16(rows, off, 0, 0);
+        else if constexpr (V == 2) w[0] = __builtin_amdgcn_raw_buffer_load_b32(rows, off, 0, 0);
+        else if constexpr (V == 4) { const u32x2 r = __builtin_amdgcn_raw_buffer_load_b64(rows, off, 0, 0); w[0] = r[0]; w[1] = r[1]; }
+        else { const u32x4 r = __builtin_amdgcn_raw_buffer_load_b128(rows, off, 0, 0); w[0] = r[0]; w[1] = r[1]; w[2] = r[2]; w[3] = r[3]; }
+    }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < NW; ++i) w[i] = 0;
     }
     __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
 };
+constexpr uint32_t NOWHERE = 0x80000000u, NOWHERE_FROM = 0x7fffffffu;    // an offset that a buffer's loads answer with zero, and where these begin
 template <int V> struct Raw<bf16, V, false> {
     uint32_t w[V];
     // (the first n)
     __device__ __forceinline__ void load(const bf16* p, int n) {
 #pragma unroll
         for (int i = 0; i < V; ++i) w[i] = i < n ? p[i].x : 0;
+    }
+    template <typename R> __device__ __forceinline__ void load(R rows, uint32_t off, int n) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = __builtin_amdgcn_raw_buffer_load_b16(rows, i < n ? off + 2 * i : NOWHERE, 0, 0);
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -94,6 +108,23 @@ template <int V, bool VEC> struct Raw<float, V, VEC> {
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) w[i] = i < n ? p[i] : 0.f;
+        }
+    }
+    template <typename R> __device__ __forceinline__ void load(R rows, uint32_t off, int n) {
+        if constexpr (VEC && V % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+                const u32x4 r = __builtin_amdgcn_raw_buffer_load_b128(rows, off + 4 * i, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[i + j] = __uint_as_float(r[j]);
+            }
+        } else if constexpr (VEC && V == 2) {
+            const u32x2 r = __builtin_amdgcn_raw_buffer_load_b64(rows, off, 0, 0);
+            w[0] = __uint_as_float(r[0]);
+            w[1] = __uint_as_float(r[1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows, i < n ? off + 4 * i : NOWHERE, 0, 0));
         }
     }
     __device__ __forceinline__ void clear() {
@@ -133,12 +164,12 @@ __device__ __forceinline__ void st_states(float* p, f32x4 x, int n, bool whole) 
         if (j < n) p[j] = x[j];
 }
 
-// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) <= 1, and log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3: the series of artanh up to s^15
-// leaves 2 s^17 / 17 <= 1e-9, also relative to the result.  No logarithm, whose hardware form loses what is small beside one.
-template <typename T> __device__ __forceinline__ float softplus(float v) {
-    const float e = exp_t<T>(-fabsf(v)), s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
-    float r = 2.f / 15.f;
-    r = __builtin_fmaf(r, q, 2.f / 13.f);
+// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) <= 1, and log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3: the series of artanh up to s^13
+// leaves 2 s^15 / 15, less than a quarter of a rounding of the result.  No logarithm, whose hardware form loses what is small beside one.
+template <typename T> __device__ __forceinline__ float softplus(float v, float& e) {
+    e = exp_t<T>(-fabsf(v));
+    const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+    float r = 2.f / 13.f;
     r = __builtin_fmaf(r, q, 2.f / 11.f);
     r = __builtin_fmaf(r, q, 2.f / 9.f);
     r = __builtin_fmaf(r, q, 2.f / 7.f);
@@ -147,6 +178,8 @@ template <typename T> __device__ __forceinline__ float softplus(float v) {
     r = __builtin_fmaf(r, q, 2.f);
     return fmaxf(v, 0.f) + s * r;
 }
+// its derivative, from that exponential
+__device__ __forceinline__ float softplus_slope(float v, float e) { return (v < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e); }
 template <typename T, int N> __device__ __forceinline__ void sigmoid_each(const float (&x)[N], float (&s)[N]) {
     float e[N];
 #pragma unroll
@@ -161,6 +194,19 @@ __device__ __forceinline__ int xcd_share(int id, int total) {
     const int xcd = id & 7, q = total >> 3, r = total & 7;
     return xcd * q + min(xcd, r) + (id >> 3);
 }
+
+// A wave's rows of an operand, tile after tile: the address of its first token's and how far the next tile's are.  (Formed anew in every tile the products
+// of strides are some 150 scalar instructions, as long as half of the vector ones.)
+template <typename T> struct Cursor {
+    const T* p;
+    long long step;
+    __device__ __forceinline__ Cursor(const T* first, long long s) : p(first), step(s) {}
+    // (opaque: the compiler would otherwise go back to products of the tile's number)
+    __device__ __forceinline__ void next() { p += step; asm("" : "+s"(p)); }
+    // The rows from there on: loads at NOWHERE give zero, which lanes without a token or a channel ask for.  (Under a condition instead every loaded register has a zero
+    // beside it that lives through the loop.)
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows() const { return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, NOWHERE_FROM, 0x00027000); }
+};
 
 // Where a lane stands: as a scanner (channel c, states 4 q .. 4 q + 3) and as a carrier of operands and results (token tok of the piece, V channels from ch)
 template <int LPC, int TOKENS> struct ScanLane {
@@ -182,25 +228,27 @@ template <int LPC, int TOKENS> struct ScanLane {
         dv = d0 + ch;
         carried = min(max(size - first - ch, 0), V);             // channels of these V that there are
     }
+    // bytes from the wave's first token's row, at channel d0, to this carrier's channels of its token
+    __device__ __forceinline__ uint32_t offset(long long row, int size) const { return ((uint32_t)tok * (uint32_t)row + (uint32_t)ch) * (uint32_t)size; }
 };
 
 // B or C of a wave's piece, its tokens x 4 LPC states, as fp32 in LDS: [tok][quad]
 template <typename T, int LPC, int TOKENS, bool VEC> struct StatesOf {
     static constexpr int PIECES = TOKENS * LPC < 64 ? 1 : TOKENS * LPC / 64;
     Raw<T, 4, VEC> r[PIECES];
-    __device__ __forceinline__ void load(const T* base, long long row, int tokens, int S) {
+    __device__ __forceinline__ void load(const Cursor<T>& base, uint32_t row, int tokens, int S) {
+        const auto rows = base.rows();
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int at = i * 64 + lane_id(), t = at / LPC, s = at % LPC * 4;
-            r[i].clear();
-            if (t < tokens && s < S) r[i].load(base + t * row + s, S - s);
+            const int e = i * 64 + lane_id(), t = e / LPC, s = e % LPC * 4;
+            r[i].load(rows, t < tokens && s < S ? (t * row + s) * (uint32_t)sizeof(T) : NOWHERE, S - s);
         }
     }
     __device__ __forceinline__ void put(f32x4* lds) const {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int at = i * 64 + lane_id();
-            if (PIECES * 64 <= TOKENS * LPC || at < TOKENS * LPC) lds[at] = f32x4{r[i][0], r[i][1], r[i][2], r[i][3]};
+            const int e = i * 64 + lane_id();
+            if (PIECES * 64 <= TOKENS * LPC || e < TOKENS * LPC) lds[e] = f32x4{r[i][0], r[i][1], r[i][2], r[i][3]};
         }
     }
 };
@@ -237,7 +285,9 @@ inline int scan_plan(const hdla_scan_dims* d, ScanPlan& s) {
         if (t != HDLA_BF16 && t != HDLA_FP32) return HDLA_ERR_DTYPE;
     if (d->B < 1 || d->T < 0 || d->D < 1 || d->S < 1 || d->S > 64 || d->G < 1 || d->D % d->G || d->N < 1) return HDLA_ERR_SHAPE;
     if (d->cu_seqlens ? d->B != 1 : d->N != d->B) return HDLA_ERR_SEQ;
-    if (d->T > (1 << 30) || d->D > (1 << 24)) return HDLA_ERR_SHAPE;
+    if (d->T > (1 << 30) || d->D > ROW_MOST) return HDLA_ERR_SHAPE;
+    for (long long r : {d->x_row, d->dt_row, d->z_row, d->B_row, d->C_row})
+        if (r < 0 || r > ROW_MOST) return HDLA_ERR_SHAPE;
     s.lpc = lanes_of(d->S);
     const int channels = 64 / s.lpc, size = d->D / d->G;
     s.per_group = (size + channels - 1) / channels;
@@ -250,7 +300,7 @@ inline int scan_plan(const hdla_scan_dims* d, ScanPlan& s) {
 }
 // Loads of V elements (channels) and of four (states): where everything lies on multiples of them
 inline bool scan_vec(const hdla_scan_dims* d, const ScanPlan& s, const ScanArgs& a) {
-    const int es = d->dtype == HDLA_BF16 ? 2 : 4, v = std::max(1, SS_TOK / s.lpc), size = d->D / d->G;
+    const int es = d->dtype == HDLA_BF16 ? 2 : 4, v = std::min(4, 2 * SS_TOK / s.lpc), size = d->D / d->G;
     if (size % v || d->S % 4) return false;
     const int bytes = std::min(v * es, 16);
     for (const Operand* o : {&a.x, &a.dt, &a.z})

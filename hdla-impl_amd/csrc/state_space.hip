@@ -12,21 +12,21 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
     using Lane = ScanLane<LPC, TOK>;
     constexpr int CHN = Lane::CHN, V = Lane::V, TILE = W * TOK, PITCH = ss_pitch(TOK);
     static_assert(W >= 4, "a thread a state of the 64 lanes");
-    __shared__ f32x4 sP[W][64], sE[W][64], sB[W][TOK * LPC], sC[W][TOK * LPC];
-    __shared__ __attribute__((aligned(16))) float sd[W][CHN * PITCH], sx[W][CHN * PITCH];
+    // a wave's own: its arrays lie at fixed distances, so that a lane holds one address for all of them
+    struct Mine { f32x4 B[TOK * LPC], C[TOK * LPC]; float d[CHN * PITCH], x[CHN * PITCH]; };
+    struct Meet { f32x4 P[W][64], E[W][64]; };
+    __shared__ __attribute__((aligned(16))) Mine mine[W];
+    __shared__ Meet meet;
 
     const int work = xcd_share(blockIdx.x, gridDim.x), n = work / p.blocks, block = work - n * p.blocks;
-    const int w = threadIdx.x >> 6, l = lane_id(), tid = threadIdx.x;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), tid = threadIdx.x;
     const Lane L(p, block);
+    Mine& my = mine[w];
     int64_t bos = 0, eos = p.T;
     if (p.cu) packed_bounds(p.cu, n, p.T, bos, eos);
     const int len = (int)(eos - bos);
     const bool whole = (p.S & 3) == 0;
     const long long batch = p.cu ? 0 : n, row0 = p.cu ? bos : (long long)n * p.T;
-    auto start = [&](const Operand& o) { return static_cast<const T*>(o.p) + batch * o.batch + bos * o.row; };
-    const T *const x0 = start(p.x) + L.dv, *const dt0 = start(p.dt) + L.dv, *const z0 = p.z.p ? start(p.z) + L.dv : nullptr;
-    const T *const B0 = start(p.B) + L.group * p.B_group, *const C0 = start(p.C) + L.group * p.C_group;
-
     f32x4 A2 = zero4();
     float bias[V], D[V];
 #pragma unroll
@@ -37,7 +37,7 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
         bias[i] = p.bias && i < L.carried ? ld_param(p.bias, p.bias_f32, L.dv + i) : 0.f;
         D[i] = p.D && i < L.carried ? ld_param(p.D, p.D_f32, L.dv + i) : 0.f;
     }
-    // The state that enters the tile, one of the 256 states of the block a thread of the first four waves: number tid of sE's rows
+    // The state that enters the tile, one of the 256 states of the block a thread of the first four waves: number tid of meet.E's rows
     const int ec = (tid >> 2) / LPC, es = 4 * ((tid >> 2) % LPC) + (tid & 3);
     const bool chains = tid < 256, there = chains && (block % p.per_group) * CHN + ec < p.DD / p.G && es < p.S;
     const long long state = ((long long)n * p.DD + L.d0 + ec) * p.S + es;
@@ -45,17 +45,22 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
 
     Raw<T, V, VEC> rx, rdt, rz;
     StatesOf<T, LPC, TOK, VEC> rB, rC;
+    const long long first = bos + w * TOK;
+    Cursor<T> cx(row_of<T>(p.x, batch, first) + L.d0, p.x.row * TILE), cdt(row_of<T>(p.dt, batch, first) + L.d0, p.dt.row * TILE),
+        cz(row_of<T>(p.z, batch, first) + L.d0, p.z.row * TILE), cB(row_of<T>(p.B, batch, first) + L.group * p.B_group, p.B.row * TILE),
+        cC(row_of<T>(p.C, batch, first) + L.group * p.C_group, p.C.row * TILE),
+        cy(static_cast<const T*>(p.y) + (row0 + w * TOK) * p.DD + L.d0, (long long)p.DD * TILE);
+    const uint32_t ox = L.offset(p.x.row, sizeof(T)), odt = L.offset(p.dt.row, sizeof(T)), oz = L.offset(p.z.row, sizeof(T)), oy = L.offset(p.DD, sizeof(T));
     auto request = [&](int t0) __attribute__((always_inline)) {
         const int tokens = min(max(len - t0, 0), TOK);
-        rx.clear(); rdt.clear(); rz.clear();
-        if (L.tok < tokens && L.carried > 0) {
-            const long long t = t0 + L.tok;
-            rx.load(x0 + t * p.x.row, L.carried);
-            rdt.load(dt0 + t * p.dt.row, L.carried);
-            if (z0) rz.load(z0 + t * p.z.row, L.carried);
-        }
-        rB.load(B0 + (long long)t0 * p.B.row, p.B.row, tokens, p.S);
-        rC.load(C0 + (long long)t0 * p.C.row, p.C.row, tokens, p.S);
+        const bool live = L.tok < tokens && L.carried > 0;
+        rx.load(cx.rows(), live ? ox : NOWHERE, L.carried);
+        rdt.load(cdt.rows(), live ? odt : NOWHERE, L.carried);
+        if (p.z.p) rz.load(cz.rows(), live ? oz : NOWHERE, L.carried);
+        else rz.clear();
+        rB.load(cB, (uint32_t)p.B.row, tokens, p.S);
+        rC.load(cC, (uint32_t)p.C.row, tokens, p.S);
+        cx.next(); cdt.next(); cz.next(); cB.next(); cC.next();
     };
     request(w * TOK);
     for (int tile = 0; tile < len; tile += TILE) {
@@ -65,85 +70,95 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
         for (int i = 0; i < V; ++i) {
             x[i] = rx[i];
             z[i] = rz[i];
-            const float v = rdt[i] + bias[i], delta = L.tok < tokens ? (p.softplus ? softplus<T>(v) : v) : 0.f;
+            float e;
+            const float v = rdt[i] + bias[i], delta = L.tok < tokens ? (p.softplus ? softplus<T>(v, e) : v) : 0.f;
             if (L.tok < TOK) {
-                sd[w][(L.ch + i) * PITCH + L.tok] = delta;
-                sx[w][(L.ch + i) * PITCH + L.tok] = delta * x[i];
+                my.d[(L.ch + i) * PITCH + L.tok] = delta;
+                my.x[(L.ch + i) * PITCH + L.tok] = delta * x[i];
             }
         }
-        rB.put(sB[w]);
-        rC.put(sC[w]);
+        rB.put(my.B);
+        rC.put(my.C);
         request(t0 + TILE);
         wave_lds_fence();
         // from zero: the decays stay in registers
-        f32x4 a[TOK], E = zero4();
-        float u[TOK], sum = 0.f;
+        f32x4 a[TOK], b[TOK], E = zero4();                // decays, and what each token adds
+        float sum = 0.f;
+        const float *const mine_d = &my.d[L.c * PITCH], *const mine_x = &my.x[L.c * PITCH];
+        float dl = mine_d[0], dx = mine_x[0];
+        b[0] = my.B[L.q];
 #pragma unroll
-        for (int k = 0; k < TOK; k += 4) {
-            const f32x4 dl = *reinterpret_cast<const f32x4*>(&sd[w][L.c * PITCH + k]), dx = *reinterpret_cast<const f32x4*>(&sx[w][L.c * PITCH + k]);
+        for (int k = 0; k < TOK; ++k) {
+            // (the next token's operands are on their way while this one's are worked on)
+            float dl1 = 0.f, dx1 = 0.f;
+            if (k + 1 < TOK) { dl1 = mine_d[k + 1]; dx1 = mine_x[k + 1]; b[k + 1] = my.B[(k + 1) * LPC + L.q]; }
+            sum += dl;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4 b = sB[w][(k + i) * LPC + L.q];
-                u[k + i] = dx[i];
-                sum += dl[i];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    a[k + i][j] = __builtin_amdgcn_exp2f(dl[i] * A2[j]);
-                    E[j] = __builtin_fmaf(a[k + i][j], E[j], dx[i] * b[j]);
-                }
-                apart();
+            for (int j = 0; j < 4; ++j) {
+                a[k][j] = __builtin_amdgcn_exp2f(dl * A2[j]);
+                b[k][j] *= dx;
+                E[j] = __builtin_fmaf(a[k][j], E[j], b[k][j]);
             }
+            dl = dl1;
+            dx = dx1;
+            apart();
         }
         f32x4 P;
 #pragma unroll
         for (int j = 0; j < 4; ++j) P[j] = __builtin_amdgcn_exp2f(sum * A2[j]);
-        sP[w][l] = P;
-        sE[w][l] = E;
+        meet.P[w][l] = P;
+        meet.E[w][l] = E;
         __syncthreads();
         if (chains) {
-            float* const e = reinterpret_cast<float*>(sE) + tid;
-            const float* const f = reinterpret_cast<const float*>(sP) + tid;
-            float ends[W], decays[W];
+            float* const e = reinterpret_cast<float*>(meet.E) + tid;
+            const float* const f = reinterpret_cast<const float*>(meet.P) + tid;
 #pragma unroll
-            for (int i = 0; i < W; ++i) { ends[i] = e[i * 256]; decays[i] = f[i * 256]; }
+            for (int k = 0; k < W; k += 4) {
+                float ends[4], decays[4];
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-                e[i * 256] = enters;
-                enters = __builtin_fmaf(decays[i], enters, ends[i]);
+                for (int i = 0; i < 4; ++i) { ends[i] = e[(k + i) * 256]; decays[i] = f[(k + i) * 256]; }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    e[(k + i) * 256] = enters;
+                    enters = __builtin_fmaf(decays[i], enters, ends[i]);
+                }
             }
         }
         __syncthreads();
-        f32x4 h = sE[w][l];
+        f32x4 h = meet.E[w][l];
         if (p.ckpt && t0 % SS_CKPT == 0 && tokens > 0)
             *reinterpret_cast<f32x4*>(p.ckpt + (((ckpt_slot(p, n, bos) + t0 / SS_CKPT) * p.blocks + block) * 64 + l) * 4) = h;
         float y[TOK];
+        f32x4 cc = my.C[L.q];
 #pragma unroll
         for (int k = 0; k < TOK; ++k) {
-            const f32x4 b = sB[w][k * LPC + L.q], cc = sC[w][k * LPC + L.q];
+            const f32x4 c1 = k + 1 < TOK ? my.C[(k + 1) * LPC + L.q] : zero4();
             float s = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                h[j] = __builtin_fmaf(a[k][j], h[j], u[k] * b[j]);
+                h[j] = __builtin_fmaf(a[k][j], h[j], b[k][j]);
                 s = __builtin_fmaf(h[j], cc[j], s);
             }
             y[k] = s;
+            cc = c1;
             apart();
         }
         sum_channel<LPC>(y);
         if (L.q == 0) {
 #pragma unroll
-            for (int k = 0; k < TOK; k += 4) *reinterpret_cast<f32x4*>(&sd[w][L.c * PITCH + k]) = f32x4{y[k], y[k + 1], y[k + 2], y[k + 3]};
+            for (int k = 0; k < TOK; k += 4) *reinterpret_cast<f32x4*>(&my.d[L.c * PITCH + k]) = f32x4{y[k], y[k + 1], y[k + 2], y[k + 3]};
         }
         wave_lds_fence();
         float o[V], g[V];
-        if (z0) sigmoid_each<T, V>(z, g);
+        if (p.z.p) sigmoid_each<T, V>(z, g);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            o[i] = __builtin_fmaf(D[i], x[i], sd[w][(L.ch + i) * PITCH + min(L.tok, TOK - 1)]);
-            if (z0) o[i] *= z[i] * g[i];
+            o[i] = __builtin_fmaf(D[i], x[i], my.d[(L.ch + i) * PITCH + min(L.tok, TOK - 1)]);
+            if (p.z.p) o[i] *= z[i] * g[i];
         }
         if (L.tok < tokens && L.carried > 0)
-            st_values<T, V, VEC>(static_cast<T*>(p.y) + (row0 + t0 + L.tok) * p.DD + L.dv, o, L.carried);
+            st_values<T, V, VEC>(at(const_cast<T*>(cy.p), oy), o, L.carried);
+        cy.next();
         wave_lds_fence();                                 // the next tile's operands go where y is
     }
     if (there && p.ht) p.ht[state] = enters;
@@ -173,7 +188,8 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs p, int lpc_log2
             C[j] = elem(p.C, g * p.C_group + 4 * q + j);
         }
     }
-    const float delta = p.softplus ? softplus<T>(v) : v;
+    float e;
+    const float delta = p.softplus ? softplus<T>(v, e) : v;
     float y = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -205,7 +221,7 @@ template <typename T> static hipError_t launch_scan(const ScanArgs& a, const Sca
 #define HDLA_SCAN_CASE(LPCV)                                                          \
     case LPCV:                                                                        \
         if (few) launch_tokens<T, LPCV, SS_TOK, 4>(a, s.vec, st);                             \
-        else launch_tokens<T, LPCV, SS_TOK, 8>(a, s.vec, st);                                 \
+        else launch_tokens<T, LPCV, LPCV == 2 ? SS_TOK : 2 * SS_TOK, 8>(a, s.vec, st);                                 \
         break;
         HDLA_SCAN_CASE(2)
         HDLA_SCAN_CASE(4)

@@ -27,12 +27,16 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
     using Lane = ScanLane<LPC, TOK>;
     constexpr int CHN = Lane::CHN, V = Lane::V, TILE = W * TOK, PITCH = ss_pitch(TOK);
     static_assert(W >= 8 && TILE % SS_CKPT == 0, "a thread a state for either chain; a tile begins where a state is left");
-    __shared__ f32x4 sP[W][64], sE[W][64], sG[W][64], sB[W][TOK * LPC], sC[W][TOK * LPC];
-    __shared__ __attribute__((aligned(16))) float sd[W][CHN * PITCH], sx[W][CHN * PITCH], se[W][CHN * PITCH], sy[W][CHN * PITCH];
+    // a wave's own: its arrays lie at fixed distances, so that a lane holds one address for all of them
+    struct Mine { f32x4 B[TOK * LPC], C[TOK * LPC]; float d[CHN * PITCH], x[CHN * PITCH], e[CHN * PITCH], y[CHN * PITCH]; };
+    struct Meet { f32x4 P[W][64], E[W][64], G[W][64]; };
+    __shared__ __attribute__((aligned(16))) Mine mine[W];
+    __shared__ Meet meet;
 
     const int work = xcd_share(blockIdx.x, gridDim.x), slot = work / p.blocks, block = work - slot * p.blocks;
-    const int w = threadIdx.x >> 6, l = lane_id(), tid = threadIdx.x;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), tid = threadIdx.x;
     const Lane L(p, block);
+    Mine& my = mine[w];
     f32x4 A2 = zero4(), dA = zero4();
     float bias[V], D[V], dD[V], dbias[V];
 #pragma unroll
@@ -53,131 +57,155 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
         if (p.cu) packed_bounds(p.cu, n, p.T, bos, eos);
         const int len = (int)(eos - bos);
         const long long batch = p.cu ? 0 : n, row0 = p.cu ? bos : (long long)n * p.T;
-        auto start = [&](const Operand& o) { return static_cast<const T*>(o.p) + batch * o.batch + bos * o.row; };
-        const T *const x0 = start(p.x) + L.dv, *const dt0 = start(p.dt) + L.dv, *const z0 = p.z.p ? start(p.z) + L.dv : nullptr;
-        const T *const B0 = start(p.B) + L.group * p.B_group, *const C0 = start(p.C) + L.group * p.C_group;
-        const T* const dy0 = static_cast<const T*>(p.dy) + row0 * p.DD + L.dv;
         const long long state = ((long long)n * p.DD + L.d0 + ec) * p.S + es;
         float enters = backwards && there && p.dht ? p.dht[state] : 0.f;
 
+        const int tiles = (len + TILE - 1) / TILE;
+        const long long first = bos + (long long)(tiles - 1) * TILE + w * TOK, frow = row0 + (long long)(tiles - 1) * TILE + w * TOK;
+        Cursor<T> cx(row_of<T>(p.x, batch, first) + L.d0, -p.x.row * TILE), cdt(row_of<T>(p.dt, batch, first) + L.d0, -p.dt.row * TILE),
+            cz(row_of<T>(p.z, batch, first) + L.d0, -p.z.row * TILE), cB(row_of<T>(p.B, batch, first) + L.group * p.B_group, -p.B.row * TILE),
+            cC(row_of<T>(p.C, batch, first) + L.group * p.C_group, -p.C.row * TILE),
+            cdy(static_cast<const T*>(p.dy) + frow * p.DD + L.d0, -(long long)p.DD * TILE);
+        long long at_row = frow * p.DD + L.d0;            // dy and the gradients lie alike
+        const uint32_t ox = L.offset(p.x.row, sizeof(T)), odt = L.offset(p.dt.row, sizeof(T)), oz = L.offset(p.z.row, sizeof(T)), oy = L.offset(p.DD, sizeof(T));
         Raw<T, V, VEC> rx, rdt, rz, rdy;
         StatesOf<T, LPC, TOK, VEC> rB, rC;
         auto request = [&](int t0) __attribute__((always_inline)) {
             const int tokens = t0 < 0 ? 0 : min(max(len - t0, 0), TOK);
-            rx.clear(); rdt.clear(); rz.clear(); rdy.clear();
-            if (L.tok < tokens && L.carried > 0) {
-                const long long t = t0 + L.tok;
-                rx.load(x0 + t * p.x.row, L.carried);
-                rdt.load(dt0 + t * p.dt.row, L.carried);
-                if (z0) rz.load(z0 + t * p.z.row, L.carried);
-                rdy.load(dy0 + t * p.DD, L.carried);
-            }
-            rB.load(B0 + (long long)t0 * p.B.row, p.B.row, tokens, p.S);
-            rC.load(C0 + (long long)t0 * p.C.row, p.C.row, tokens, p.S);
+            const bool live = L.tok < tokens && L.carried > 0;
+            rx.load(cx.rows(), live ? ox : NOWHERE, L.carried);
+            rdt.load(cdt.rows(), live ? odt : NOWHERE, L.carried);
+            if (p.z.p) rz.load(cz.rows(), live ? oz : NOWHERE, L.carried);
+            else rz.clear();
+            rdy.load(cdy.rows(), live ? oy : NOWHERE, L.carried);
+            rB.load(cB, (uint32_t)p.B.row, tokens, p.S);
+            rC.load(cC, (uint32_t)p.C.row, tokens, p.S);
+            cx.next(); cdt.next(); cz.next(); cdy.next(); cB.next(); cC.next();
         };
-        const int tiles = (len + TILE - 1) / TILE;
         request((tiles - 1) * TILE + w * TOK);
         for (int tile = tiles - 1; tile >= 0; --tile) {
             const int t0 = tile * TILE + w * TOK, tokens = min(max(len - t0, 0), TOK);
             const float left = forwards ? p.ckpt[((ckpt_slot(p, n, bos) + tile * (TILE / SS_CKPT)) * p.blocks + block) * 256 + e] : 0.f;
-            float x[V], z[V], dy[V], v[V], gz[V], delta[V], ee[V];
+            float x[V], z[V], dy[V], v[V], ev[V], gz[V], delta[V], ee[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) { x[i] = rx[i]; z[i] = rz[i]; dy[i] = rdy[i]; v[i] = rdt[i] + bias[i]; }
-            if (z0) sigmoid_each<T, V>(z, gz);
+            if (p.z.p) sigmoid_each<T, V>(z, gz);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                delta[i] = L.tok < tokens ? (p.softplus ? softplus<T>(v[i]) : v[i]) : 0.f;
-                ee[i] = z0 ? dy[i] * (z[i] * gz[i]) : dy[i];
-                const int at = (L.ch + i) * PITCH + L.tok;
+                delta[i] = L.tok < tokens ? (p.softplus ? softplus<T>(v[i], ev[i]) : v[i]) : 0.f;
+                ee[i] = p.z.p ? dy[i] * (z[i] * gz[i]) : dy[i];
+                const int place = (L.ch + i) * PITCH + L.tok;
                 if (L.tok < TOK) {
-                    sd[w][at] = delta[i];
-                    sx[w][at] = delta[i] * x[i];
-                    se[w][at] = ee[i];
+                    my.d[place] = delta[i];
+                    my.x[place] = delta[i] * x[i];
+                    my.e[place] = ee[i];
                 }
             }
-            rB.put(sB[w]);
-            rC.put(sC[w]);
+            rB.put(my.B);
+            rC.put(my.C);
             request(t0 - TILE);
             wave_lds_fence();
             f32x4 a[TOK], E = zero4(), G = zero4();
-            const float *const mine_d = &sd[w][L.c * PITCH], *const mine_x = &sx[w][L.c * PITCH], *const mine_e = &se[w][L.c * PITCH];
+            const float *const mine_d = &my.d[L.c * PITCH], *const mine_x = &my.x[L.c * PITCH], *const mine_e = &my.e[L.c * PITCH];
             float sum = 0.f;
+            // (in all the walks: the next token's operands are on their way while this one's are worked on)
+            {
+                f32x4 b = my.B[L.q];
+                float dl = mine_d[0], u = mine_x[0];
 #pragma unroll
-            for (int k = 0; k < TOK; ++k) {
-                const f32x4 b = sB[w][k * LPC + L.q];
-                const float dl = mine_d[k], u = mine_x[k];
-                sum += dl;
+                for (int k = 0; k < TOK; ++k) {
+                    f32x4 b1;
+                    float dl1, u1;
+                    if (k + 1 < TOK) { b1 = my.B[(k + 1) * LPC + L.q]; dl1 = mine_d[k + 1]; u1 = mine_x[k + 1]; }
+                    sum += dl;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    a[k][j] = __builtin_amdgcn_exp2f(dl * A2[j]);
-                    E[j] = __builtin_fmaf(a[k][j], E[j], u * b[j]);
+                    for (int j = 0; j < 4; ++j) {
+                        a[k][j] = __builtin_amdgcn_exp2f(dl * A2[j]);
+                        E[j] = __builtin_fmaf(a[k][j], E[j], u * b[j]);
+                    }
+                    apart();
+                    if (k + 1 < TOK) { b = b1; dl = dl1; u = u1; }
                 }
-                apart();
             }
+            {
+                f32x4 cc = my.C[(TOK - 1) * LPC + L.q];
+                float et = mine_e[TOK - 1];
 #pragma unroll
-            for (int k = TOK - 1; k >= 0; --k) {
-                const f32x4 cc = sC[w][k * LPC + L.q];
-                const float ev = mine_e[k];
+                for (int k = TOK - 1; k >= 0; --k) {
+                    f32x4 c1;
+                    float e1;
+                    if (k) { c1 = my.C[(k - 1) * LPC + L.q]; e1 = mine_e[k - 1]; }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) G[j] = a[k][j] * __builtin_fmaf(cc[j], ev, G[j]);
-                apart();
+                    for (int j = 0; j < 4; ++j) G[j] = a[k][j] * __builtin_fmaf(cc[j], et, G[j]);
+                    apart();
+                    if (k) { cc = c1; et = e1; }
+                }
             }
             f32x4 P;
 #pragma unroll
             for (int j = 0; j < 4; ++j) P[j] = __builtin_amdgcn_exp2f(sum * A2[j]);
-            sP[w][l] = P;
-            sE[w][l] = E;
-            sG[w][l] = G;
+            meet.P[w][l] = P;
+            meet.E[w][l] = E;
+            meet.G[w][l] = G;
             __syncthreads();
             if (tid < 512) {
-                float* const at = reinterpret_cast<float*>(forwards ? sE : sG) + e;
-                const float* const f = reinterpret_cast<const float*>(sP) + e;
+                float* const ends_at = reinterpret_cast<float*>(forwards ? meet.E : meet.G) + e;
+                const float* const f = reinterpret_cast<const float*>(meet.P) + e;
                 float ends[W], decays[W];
 #pragma unroll
-                for (int i = 0; i < W; ++i) { ends[i] = at[i * 256]; decays[i] = f[i * 256]; }
+                for (int i = 0; i < W; ++i) { ends[i] = ends_at[i * 256]; decays[i] = f[i * 256]; }
                 if (forwards) {
                     enters = left;
 #pragma unroll
                     for (int i = 0; i < W; ++i) {
-                        at[i * 256] = enters;
+                        ends_at[i * 256] = enters;
                         enters = __builtin_fmaf(decays[i], enters, ends[i]);
                     }
                 } else {
 #pragma unroll
                     for (int i = W - 1; i >= 0; --i) {
-                        at[i * 256] = enters;
+                        ends_at[i * 256] = enters;
                         enters = __builtin_fmaf(decays[i], enters, ends[i]);
                     }
                 }
             }
             __syncthreads();
-            const f32x4 first = sE[w][l];
-            G = sG[w][l];
+            const f32x4 first = meet.E[w][l];
+            G = meet.G[w][l];
             f32x4 h[TOK];
+            {
+                f32x4 b = my.B[L.q], cc = my.C[L.q];
+                float u = mine_x[0];
 #pragma unroll
-            for (int k = 0; k < TOK; ++k) {
-                const f32x4 b = sB[w][k * LPC + L.q], cc = sC[w][k * LPC + L.q];
-                const float u = mine_x[k];
-                float y[1] = {0.f};
+                for (int k = 0; k < TOK; ++k) {
+                    f32x4 b1, c1;
+                    float u1;
+                    if (k + 1 < TOK) { b1 = my.B[(k + 1) * LPC + L.q]; c1 = my.C[(k + 1) * LPC + L.q]; u1 = mine_x[k + 1]; }
+                    float y[1] = {0.f};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    h[k][j] = __builtin_fmaf(a[k][j], k ? h[k - 1][j] : first[j], u * b[j]);
-                    y[0] = __builtin_fmaf(h[k][j], cc[j], y[0]);
+                    for (int j = 0; j < 4; ++j) {
+                        h[k][j] = __builtin_fmaf(a[k][j], k ? h[k - 1][j] : first[j], u * b[j]);
+                        y[0] = __builtin_fmaf(h[k][j], cc[j], y[0]);
+                    }
+                    sum_channel<LPC>(y);
+                    my.y[L.c * PITCH + k] = y[0];        // (the same from all lanes of the channel)
+                    apart();
+                    if (k + 1 < TOK) { b = b1; cc = c1; u = u1; }
                 }
-                sum_channel<LPC>(y);
-                sy[w][L.c * PITCH + k] = y[0];            // (the same from all lanes of the channel)
-                apart();
             }
             wave_lds_fence();                             // B and C are read again, not kept
+            f32x4 b = my.B[(TOK - 1) * LPC + L.q], cc = my.C[(TOK - 1) * LPC + L.q];
+            float dl = mine_d[TOK - 1], u = mine_x[TOK - 1], et = mine_e[TOK - 1];
 #pragma unroll
             for (int k = TOK - 1; k >= 0; --k) {
-                const f32x4 b = sB[w][k * LPC + L.q], cc = sC[w][k * LPC + L.q];
-                const float dl = mine_d[k], u = mine_x[k], ev = mine_e[k];
+                f32x4 b1, c1;
+                float dl1, u1, e1;
+                if (k) { b1 = my.B[(k - 1) * LPC + L.q]; c1 = my.C[(k - 1) * LPC + L.q]; dl1 = mine_d[k - 1]; u1 = mine_x[k - 1]; e1 = mine_e[k - 1]; }
                 float s[2] = {0.f, 0.f}, db[4], dc[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float g = __builtin_fmaf(cc[j], ev, G[j]);
-                    dc[j] = ev * h[k][j];
+                    const float g = __builtin_fmaf(cc[j], et, G[j]);
+                    dc[j] = et * h[k][j];
                     db[j] = g * u;
                     s[0] = __builtin_fmaf(g, b[j], s[0]);
                     G[j] = a[k][j] * g;
@@ -192,37 +220,38 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
                 if constexpr (LPC < 4) { f0 += dpp0<0x122>(f0); f1 += dpp0<0x122>(f1); }
                 sum_channel<LPC>(s);
                 // (what this token had there has been read: B, C, delta, delta x)
-                sd[w][L.c * PITCH + k] = s[0];
-                sx[w][L.c * PITCH + k] = s[1];
+                my.d[L.c * PITCH + k] = s[0];
+                my.x[L.c * PITCH + k] = s[1];
                 if ((l & 15) < LPC) {
-                    float* const to = reinterpret_cast<float*>(&(l < 32 ? sB : sC)[w][k * LPC + (l & 15)]) + ((l >> 4) & 1);
+                    float* const to = reinterpret_cast<float*>(&(l < 32 ? my.B : my.C)[k * LPC + (l & 15)]) + ((l >> 4) & 1);
                     to[0] = f0;
                     to[2] = f1;
                 }
                 apart();
+                if (k) { b = b1; cc = c1; dl = dl1; u = u1; et = e1; }
             }
             wave_lds_fence();
-            float ox[V], odt[V], oz[V], sv[V];
-            if (p.softplus) sigmoid_each<T, V>(v, sv);
+            float gx[V], gdt[V], gzz[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const int at = (L.ch + i) * PITCH + min(L.tok, TOK - 1);
-                const float gb = sd[w][at], ga = sx[w][at] * LN2, inner = __builtin_fmaf(D[i], x[i], sy[w][at]);
-                ox[i] = __builtin_fmaf(D[i], ee[i], gb * delta[i]);
-                odt[i] = __builtin_fmaf(gb, x[i], ga);
-                if (p.softplus) odt[i] *= sv[i];
-                if (z0) oz[i] = dy[i] * inner * (gz[i] * __builtin_fmaf(z[i], 1.f - gz[i], 1.f));
+                const int place = (L.ch + i) * PITCH + min(L.tok, TOK - 1);
+                const float gb = my.d[place], ga = my.x[place] * LN2, inner = __builtin_fmaf(D[i], x[i], my.y[place]);
+                gx[i] = __builtin_fmaf(D[i], ee[i], gb * delta[i]);
+                gdt[i] = __builtin_fmaf(gb, x[i], ga);
+                if (p.softplus) gdt[i] *= softplus_slope(v[i], ev[i]);
+                if (p.z.p) gzz[i] = dy[i] * inner * (gz[i] * __builtin_fmaf(z[i], 1.f - gz[i], 1.f));
                 if (L.tok < tokens) {
                     dD[i] = __builtin_fmaf(ee[i], x[i], dD[i]);
-                    dbias[i] += odt[i];
+                    dbias[i] += gdt[i];
                 }
             }
             if (L.tok < tokens && L.carried > 0) {
-                const long long at = (row0 + t0 + L.tok) * p.DD + L.dv;
-                st_values<T, V, VEC>(static_cast<T*>(p.dx) + at, ox, L.carried);
-                st_values<T, V, VEC>(static_cast<T*>(p.ddt) + at, odt, L.carried);
-                if (z0) st_values<T, V, VEC>(static_cast<T*>(p.dz) + at, oz, L.carried);
+                st_values<T, V, VEC>(at(static_cast<T*>(p.dx) + at_row, oy), gx, L.carried);
+                st_values<T, V, VEC>(at(static_cast<T*>(p.ddt) + at_row, oy), gdt, L.carried);
+                if (p.z.p) st_values<T, V, VEC>(at(static_cast<T*>(p.dz) + at_row, oy), gzz, L.carried);
             }
+            at_row -= (long long)TILE * p.DD;
+            asm("" : "+s"(at_row));
             // this block's part of dB and dC: [block of the group][B, C][row][group][S]
             {
                 const long long inner = (long long)p.G * p.S, half = p.rows * inner;
@@ -230,10 +259,10 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
                 constexpr int PIECES = TOK * LPC < 64 ? 1 : TOK * LPC / 64;
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {
-                    const int at = i * 64 + l, t = at / LPC, s = at % LPC * 4;
+                    const int piece = i * 64 + l, t = piece / LPC, s = piece % LPC * 4;
                     if (t < tokens && s < p.S) {
-                        st_states(to + t * inner + s, sB[w][at], p.S - s, VEC);
-                        st_states(to + half + t * inner + s, sC[w][at], p.S - s, VEC);
+                        st_states(to + t * inner + s, my.B[piece], p.S - s, VEC);
+                        st_states(to + half + t * inner + s, my.C[piece], p.S - s, VEC);
                     }
                 }
             }
@@ -243,24 +272,24 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
     }
     // what the waves have of dA, dD and d bias
     __syncthreads();
-    sE[w][l] = dA;
+    meet.E[w][l] = dA;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         // over the tokens
 #pragma unroll
         for (int m = CHN / V; m < 64; m *= 2) { dD[i] += __shfl_xor(dD[i], m); dbias[i] += __shfl_xor(dbias[i], m); }
-        if (l < CHN / V) { sd[w][L.ch + i] = dD[i]; sx[w][L.ch + i] = dbias[i]; }
+        if (l < CHN / V) { my.d[L.ch + i] = dD[i]; my.x[L.ch + i] = dbias[i]; }
     }
     __syncthreads();
     if (tid < 256) {
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < W; ++i) s += reinterpret_cast<const float*>(sE)[i * 256 + e];
+        for (int i = 0; i < W; ++i) s += reinterpret_cast<const float*>(meet.E)[i * 256 + e];
         if (there) p.part_a[((long long)slot * p.DD + L.d0 + ec) * p.S + es] = s;
     } else if (backwards && e < CHN && (block % p.per_group) * CHN + e < p.DD / p.G) {
         float s = 0.f, b = 0.f;
 #pragma unroll
-        for (int i = 0; i < W; ++i) { s += sd[i][e]; b += sx[i][e]; }
+        for (int i = 0; i < W; ++i) { s += mine[i].d[e]; b += mine[i].x[e]; }
         p.part_d[(long long)slot * p.DD + L.d0 + e] = s;
         p.part_bias[(long long)slot * p.DD + L.d0 + e] = b;
     }

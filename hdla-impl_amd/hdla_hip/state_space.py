@@ -19,6 +19,7 @@ from .utils import autocast_custom_bwd, autocast_custom_fwd
 
 _NATIVE = (torch.bfloat16, torch.float32)
 CONV_WIDTHS, MAX_STATES = (2, 3, 4), 64
+ROW_MOST = 1 << 24
 
 
 def on_one_gpu(x, *others):
@@ -29,8 +30,15 @@ def on_one_gpu(x, *others):
 
 
 def rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """A tensor whose last dimension is contiguous: itself, or a copy."""
-    return t if t is None or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    """A tensor whose last dimension is contiguous and whose tokens are no further apart than the kernels reach: itself, or a copy."""
+    if t is None or ((t.shape[-1] == 1 or t.stride(-1) == 1) and step(t, 1) <= ROW_MOST):
+        return t
+    return t.contiguous()
+
+
+def step(t, dim):
+    """Elements from one index of a dimension to the next, where there is a next."""
+    return t.stride(dim) if t.shape[dim] > 1 else 0
 
 
 def whole(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -74,7 +82,7 @@ def _not_trained(name):
 def _conv_dims(x, weight, bias, silu, n, cu):
     b, t = (x.shape[0], x.shape[1]) if x.dim() == 3 else (x.shape[0], 1)
     return _lib.HdlaConvDims(b, t, x.shape[-1], weight.shape[1], n, _lib.dtype_code(x.dtype), code(weight), code(bias), int(silu),
-                             x.stride(0), x.stride(1) if x.dim() == 3 else 0, None if cu is None else cu.data_ptr())
+                             step(x, 0), step(x, 1) if x.dim() == 3 else 0, None if cu is None else cu.data_ptr())
 
 
 def _conv_args(x, weight, bias, activation):
@@ -231,9 +239,9 @@ def short_conv_step(
 # ---- the scan --------------------------------------------------------------------------------------------------------
 def _scan_dims(x, dt, A, B, C, D, z, bias, softplus, n, cu):
     one = x.dim() == 2
-    st = lambda t: (0, 0) if t is None else (t.stride(0), 0 if one else t.stride(1))
+    st = lambda t: (0, 0) if t is None else (step(t, 0), 0 if one else step(t, 1))
     return _lib.HdlaScanDims(x.shape[0], 1 if one else x.shape[1], x.shape[-1], A.shape[1], B.shape[-2], n, _lib.dtype_code(x.dtype), code(A), code(D), code(bias),
-                             int(softplus), *st(x), *st(dt), *st(z), *st(B), B.stride(-2), *st(C), C.stride(-2), None if cu is None else cu.data_ptr())
+                             int(softplus), *st(x), *st(dt), *st(z), *st(B), step(B, -2), *st(C), step(C, -2), None if cu is None else cu.data_ptr())
 
 
 def _scan_args(x, dt, A, B, C, D, z, dt_bias):

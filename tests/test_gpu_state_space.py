@@ -128,6 +128,16 @@ def test_channels_first_and_expanded_inputs():
     compare(low, ref, dy, dh, True, v=v)
 
 
+def test_strides_of_dimensions_of_one_and_tokens_far_apart():
+    low, ref, dy, dh = make(23, 1, 3, 16, 16, 1, torch.bfloat16)
+    v = put(low)
+    far = torch.zeros(2 * ((1 << 24) + 8) + 16, dtype=torch.bfloat16, device=DEV).as_strided((1, 3, 16), (0, (1 << 24) + 8, 1))
+    far.copy_(low["x"])
+    v["x"] = far.detach().requires_grad_()
+    v["dt"] = torch.empty(1, dtype=torch.bfloat16, device=DEV).expand(1 << 24).new_zeros(3 * 16).as_strided((1, 3, 16), (5, 16, 1)).copy_(low["dt"]).detach().requires_grad_()
+    compare(low, ref, dy, dh, True, v=v)
+
+
 def test_bf16_parameters_and_mixed_types():
     low, ref, dy, dh = make(13, 1, 70, 16, 16, 1, torch.bfloat16, pdtype=torch.bfloat16)
     compare(low, ref, dy, dh, True)
