@@ -25,6 +25,7 @@
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -35,6 +36,7 @@
 #include <vector>
 
 #include "../../include/hdla_hip.h"
+#include "../../include/hdla_state_space.h"
 #include "host_path.h"
 
 namespace {
@@ -55,6 +57,9 @@ struct Api {
     HDLA_FN(weight_grad); HDLA_FN(weight_grad_workspace_bytes); HDLA_FN(weight_grad_pair); HDLA_FN(weight_grad_pair_workspace_bytes);
     HDLA_FN(normalize_bwd_later); HDLA_FN(layer_up_wgrad_later); HDLA_FN(run_sums);
     HDLA_FN(layer_step); HDLA_FN(rows_gemm_norm);
+    HDLA_FN(short_conv_fwd); HDLA_FN(short_conv_workspace_bytes); HDLA_FN(short_conv_bwd); HDLA_FN(short_conv_step);
+    HDLA_FN(scan_states_bytes); HDLA_FN(scan_fwd); HDLA_FN(scan_workspace_bytes); HDLA_FN(scan_bwd); HDLA_FN(scan_step);
+    HDLA_FN(block_norm_fwd); HDLA_FN(block_norm_workspace_bytes); HDLA_FN(block_norm_bwd);
 #undef HDLA_FN
 } api;
 PyObject* error_class = nullptr;                 // _lib.HdlaError
@@ -1202,6 +1207,8 @@ PyObject* py_layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+#include "native_state_space.inc"
+
 // ---- module ----------------------------------------------------------------------------------------------------------
 // bind(handle of libhdla_hip.so, HdlaError, torch.OutOfMemoryError)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -1223,6 +1230,9 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HDLA_FN(weight_grad) HDLA_FN(weight_grad_workspace_bytes) HDLA_FN(weight_grad_pair) HDLA_FN(weight_grad_pair_workspace_bytes)
     HDLA_FN(normalize_bwd_later) HDLA_FN(layer_up_wgrad_later) HDLA_FN(run_sums)
     HDLA_FN(rows_gemm_norm)
+    HDLA_FN(short_conv_fwd) HDLA_FN(short_conv_workspace_bytes) HDLA_FN(short_conv_bwd) HDLA_FN(short_conv_step)
+    HDLA_FN(scan_states_bytes) HDLA_FN(scan_fwd) HDLA_FN(scan_workspace_bytes) HDLA_FN(scan_bwd) HDLA_FN(scan_step)
+    HDLA_FN(block_norm_fwd) HDLA_FN(block_norm_workspace_bytes) HDLA_FN(block_norm_bwd)
 #undef HDLA_FN
     Py_INCREF(a[1]);
     Py_XDECREF(error_class);
@@ -1238,7 +1248,8 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {
     HDLA_DEF("bind", py_bind), HDLA_DEF("chunk", py_chunk), HDLA_DEF("chunk_hdla", py_chunk_hdla), HDLA_DEF("recurrent", py_recurrent),
     HDLA_DEF("recurrent_hdla", py_recurrent_hdla), HDLA_DEF("normalize", py_normalize), HDLA_DEF("layer", py_layer), HDLA_DEF("forget", py_forget), HDLA_DEF("passed", py_passed),
-    HDLA_DEF("kept_room", py_kept_room), {nullptr, nullptr, 0, nullptr}};
+    HDLA_DEF("short_conv", py_short_conv), HDLA_DEF("short_conv_step", py_short_conv_step), HDLA_DEF("state_space_scan", py_state_space_scan),
+    HDLA_DEF("state_space_step", py_state_space_step), HDLA_DEF("block_norm", py_block_norm), HDLA_DEF("kept_room", py_kept_room), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -217,6 +217,7 @@ class _NoNative:
         return None
 
     chunk = chunk_hdla = recurrent = recurrent_hdla = normalize = layer = passed = _not_mine
+    short_conv = short_conv_step = state_space_scan = state_space_step = block_norm = _not_mine
 
     def forget(self, cache):
         return [None] * 4

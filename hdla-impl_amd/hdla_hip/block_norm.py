@@ -77,6 +77,9 @@ def block_norm(
 
     ``gate_act``: "sigmoid", "silu" or None (the gate multiplies as it is).  ``residual_scale``: a number, or a tensor [E] (learned).  The stream may be fp32 beside
     bf16 blocks.  E is at most 4096.  ``y`` is formed from the sum before that is rounded to the stream's type."""
+    out = _lib.native().block_norm(x, residual, weight, post_norm, post_weight, gate, gate_act, residual_scale, eps)
+    if out is not None:
+        return out
     E = x.shape[-1] if x.dim() else 0
     if E < 1:
         raise ValueError(f"x must be [..., E], got {tuple(x.shape)}")

@@ -153,6 +153,9 @@ def short_conv(
 
     ``initial_state`` holds the W - 1 inputs before each sequence (zeros without it), the returned ``final_state`` its last W - 1, both oldest first;
     ``cu_seqlens`` packs N sequences into a batch of one.  Returns ``(y, final_state)``, both in x's dtype."""
+    out = _lib.native().short_conv(x, weight, bias, activation, initial_state, output_final_state, cu_seqlens)
+    if out is not None:
+        return out
     if x.dim() != 3:
         raise ValueError(f"x must be [B, T, D], got {tuple(x.shape)}")
     silu = _conv_args(x, weight, bias, activation)
@@ -211,6 +214,9 @@ def short_conv_step(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """``short_conv`` for one token of each sequence: returns ``(y [B, D], new_state)``.  ``inplace=True`` writes the new state where ``state`` is, as
     a loop of decode steps or a captured graph wants it.  No gradients."""
+    out = _lib.native().short_conv_step(x, state, weight, bias, activation, inplace)
+    if out is not None:
+        return out
     if x.dim() != 2:
         raise ValueError(f"x must be [B, D], got {tuple(x.shape)}")
     silu = _conv_args(x, weight, bias, activation)
@@ -343,6 +349,9 @@ def state_space_scan(
 
     ``A`` is what stands in the exponent (negative where states decay).  Returns ``(y [B, T, D] in x's dtype, final_state [N, D, S] fp32 or None)``;
     ``cu_seqlens`` packs N sequences into a batch of one.  x, dt, B, C and z of different types are computed in fp32."""
+    out = _lib.native().state_space_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state, cu_seqlens)
+    if out is not None:
+        return out
     if x.dim() != 3:
         raise ValueError(f"x must be [B, T, D], got {tuple(x.shape)}")
     B, C = _scan_args(x, dt, A, B, C, D, z, dt_bias)
@@ -373,6 +382,9 @@ def state_space_step(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """``state_space_scan`` for one token of each sequence: returns ``(y [B, D], new_state [B, D, S] fp32)``.  ``inplace=True`` writes the new state where
     ``state`` is, as a loop of decode steps or a captured graph wants it.  No gradients."""
+    out = _lib.native().state_space_step(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, inplace)
+    if out is not None:
+        return out
     if x.dim() != 2:
         raise ValueError(f"x must be [B, D], got {tuple(x.shape)}")
     B, C = _scan_args(x, dt, A, B, C, D, z, dt_bias)
