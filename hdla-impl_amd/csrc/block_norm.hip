@@ -6,7 +6,7 @@
 //     dgate = du p act'(gate);   dp = du act(gate);   dpost_weight = sum dp xhat;   q = dp post_weight;  dx = (q - xhat mean(q xhat)) / rms(x)
 //
 // Streams through HBM: forward reads x, gate, residual and writes y, r; backward reads these, dy, dr and writes dx, dgate, dresidual.  A row lies in the registers
-// of one wave, or of the four waves of a workgroup where it is long, 16 bytes a lane and piece; its sums are taken across lanes without LDS (a workgroup's four through it).
+// of one wave, or of two, four or eight waves of a workgroup where it is long, 16 bytes a lane and piece; its sums are taken across lanes without LDS (several waves' through it).
 // Workgroups stride over rows: weights are read once, and the gradients of weights and scale stay in registers until a workgroup leaves one row of partial sums.
 #include "column_sums.cuh"
 #include "hdla_common.cuh"
@@ -26,18 +26,40 @@ struct BlockNormArgs {
 };
 enum { ACT_NONE, ACT_SIGMOID, ACT_SILU };
 
-// N channels from e on; beyond the row's end (it need not be a multiple of N where VEC is false) zeros
-template <typename T, int N, bool VEC> __device__ __forceinline__ void ld_row(const void* base, long long row, int E, int e, float (&f)[N]) {
-    Raw<T, N, VEC> r;
-    r.clear();
-    if (e < E) r.load(static_cast<const T*>(base) + row * E + e, E - e);
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = r[i];
-}
+// N channels of a vector from e on; beyond its end, or without one, `none`
 template <int N, bool VEC> __device__ __forceinline__ void ld_vector(const void* v, int f32, int E, int e, float none, float (&f)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = v && e + i < E ? ld_param(v, f32, e + i) : none;
+    for (int i = 0; i < N; ++i) f[i] = none;
+    if (!v || e >= E) return;
+    if constexpr (VEC) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const f32x4 r = f32 ? *reinterpret_cast<const f32x4*>(static_cast<const float*>(v) + e + i) : to_f32(ld_frag(static_cast<const bf16*>(v) + e + i));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[i + j] = r[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (e + i < E) f[i] = ld_param(v, f32, e + i);
+    }
 }
+// A lane's pieces of one row as they come from memory: 16 bytes of x's type each.  Lanes behind the row's end, and rows behind the last, ask for nothing and get zeros.
+template <typename X, int N, int NV, bool VEC> struct RowOf {
+    Raw<X, N, VEC> p[NV];
+    __device__ __forceinline__ void load(const void* base, long long row, bool live, int E, int lanes, int lane) {
+        const auto rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<X*>(static_cast<const X*>(base) + row * E), 0, NOWHERE_FROM, 0x00027000);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = (i * lanes + lane) * N;
+            p[i].load(rows, live && e < E ? e * (uint32_t)sizeof(X) : NOWHERE, E - e);
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) p[i].clear();
+    }
+};
 template <typename T, int N, bool VEC> __device__ __forceinline__ void st_row(void* base, long long row, int E, int e, const float (&f)[N]) {
     if (e < E) st_values<T, N, VEC>(static_cast<T*>(base) + row * E + e, f, E - e);
 }
@@ -57,7 +79,7 @@ template <typename T, int N> __device__ __forceinline__ void activate(int act, c
     }
 }
 
-// Sums over a row: the lanes of a wave, or (WAVES = 4) of a workgroup, whose threads all make the same calls; alternating halves of LDS, so one barrier a call
+// Sums over a row: the lanes of a wave, or of several in a workgroup, whose threads all make the same calls; alternating halves of LDS, so one barrier a call
 template <int WAVES, int N> struct RowSum {
     float* lds;
     int half = 0;
@@ -67,7 +89,7 @@ template <int WAVES, int N> struct RowSum {
             float* const s = lds + half * WAVES * N;
             if ((threadIdx.x & 63) == 0)
 #pragma unroll
-                for (int i = 0; i < N; ++i) s[(threadIdx.x >> 6) * N + i] = x[i];
+                for (int i = 0; i < N; ++i) s[(threadIdx.x >> 6) % WAVES * N + i] = x[i];
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -80,33 +102,55 @@ template <int WAVES, int N> struct RowSum {
     }
 };
 
-// x and gate of T, residual, r of S.  NV pieces of N channels a lane; WAVES waves a row
+// x and gate of T, residual, r of S.  NV pieces of N channels a lane; WAVES waves a row, a workgroup of four waves (eight of a row of eight).  A row's pieces are on
+// their way while the row before it is worked on.
+template <int WAVES> struct RowShare {
+    static constexpr int THREADS = WAVES == 8 ? 512 : 256, LANES = 64 * WAVES, ROWS = THREADS / LANES;
+    long long row, step;
+    int lane;
+    __device__ __forceinline__ RowShare() {
+        const int mine = __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+        row = (long long)blockIdx.x * ROWS + mine;
+        step = (long long)gridDim.x * ROWS;
+        lane = threadIdx.x - mine * LANES;
+    }
+    // (every wave of a workgroup makes as many turns)
+    __device__ __forceinline__ int turns(long long rows) const { return (int)((rows - (long long)blockIdx.x * ROWS + step - 1) / step); }
+};
 template <typename T, typename S, int NV, int WAVES, bool VEC>
-__global__ __launch_bounds__(WAVES == 8 ? 512 : 256) void block_norm_kernel(BlockNormArgs p) {
-    constexpr int N = 16 / sizeof(T), LANES = 64 * WAVES, ROWS = WAVES == 1 ? 4 : 1;
-    __shared__ float lds[2 * WAVES];
-    RowSum<WAVES, 1> sum{lds};
-    const int lane = threadIdx.x % LANES;
+__global__ __launch_bounds__(RowShare<WAVES>::THREADS) void block_norm_kernel(BlockNormArgs p) {
+    using Share = RowShare<WAVES>;
+    constexpr int N = 16 / sizeof(T), LANES = Share::LANES;
+    __shared__ float lds[Share::ROWS][2 * WAVES];
+    Share at;
+    RowSum<WAVES, 1> sum{lds[threadIdx.x / LANES]};
+    RowOf<T, N, NV, VEC> rx, rg;
+    RowOf<S, N, NV, VEC> rr;
+    auto request = [&](long long row) __attribute__((always_inline)) {
+        const bool live = row < p.rows;
+        rx.load(p.x, row, live, p.E, LANES, at.lane);
+        if (p.gate) rg.load(p.gate, row, live, p.E, LANES, at.lane);
+        else rg.clear();
+        if (p.residual) rr.load(p.residual, row, live, p.E, LANES, at.lane);
+        else rr.clear();
+    };
+    request(at.row);
     float w[NV][N], pw[NV][N], sc[NV][N];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int e = (i * LANES + lane) * N;
+        const int e = (i * LANES + at.lane) * N;
         ld_vector<N, VEC>(p.weight, p.w_f32, p.E, e, 1.f, w[i]);
         ld_vector<N, VEC>(p.post, p.p_f32, p.E, e, 1.f, pw[i]);
         ld_vector<N, VEC>(p.scale, p.s_f32, p.E, e, p.factor, sc[i]);
     }
-    for (long long first = (long long)blockIdx.x * ROWS; first < p.rows; first += (long long)gridDim.x * ROWS) {
-        const long long row = first + threadIdx.x / LANES;
-        const bool live = row < p.rows;
-        const int E = live ? p.E : 0;
+    for (int turn = at.turns(p.rows); turn > 0; --turn, at.row += at.step) {
+        const int E = at.row < p.rows ? p.E : 0;
         float x[NV][N], r[NV][N], g[NV][N];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int e = (i * LANES + lane) * N;
-            ld_row<T, N, VEC>(p.x, row, E, e, x[i]);
-            if (p.residual) ld_row<S, N, VEC>(p.residual, row, E, e, r[i]);
-            if (p.gate) ld_row<T, N, VEC>(p.gate, row, E, e, g[i]);
-        }
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) { x[i][j] = rx.p[i][j]; r[i][j] = rr.p[i][j]; g[i][j] = rg.p[i][j]; }
+        if (turn > 1) request(at.row + at.step);
         float inv = 1.f;
         if (p.post_norm) {
             float s[1] = {0.f};
@@ -126,8 +170,7 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256) void block_norm_kernel(Bloc
             for (int j = 0; j < N; ++j) {
                 float u = x[i][j] * inv * pw[i][j];
                 if (p.gate) u *= a[j];
-                u *= sc[i][j];
-                r[i][j] = p.residual ? r[i][j] + u : u;
+                r[i][j] = __builtin_fmaf(u, sc[i][j], r[i][j]);
                 s[0] = __builtin_fmaf(r[i][j], r[i][j], s[0]);
             }
         }
@@ -135,160 +178,172 @@ __global__ __launch_bounds__(WAVES == 8 ? 512 : 256) void block_norm_kernel(Bloc
         const float ir = 1.f / sqrtf(__builtin_fmaf(s[0], p.inv_e, p.eps));
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int e = (i * LANES + lane) * N;
+            const int e = (i * LANES + at.lane) * N;
             float y[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) y[j] = r[i][j] * ir * w[i][j];
-            st_row<T, N, VEC>(p.y, row, E, e, y);
-            st_row<S, N, VEC>(p.r, row, E, e, r[i]);
+            st_row<T, N, VEC>(p.y, at.row, E, e, y);
+            st_row<S, N, VEC>(p.r, at.row, E, e, r[i]);
         }
     }
 }
 
-// (four channels a lane and piece: their sums' registers are three times theirs. )
 template <typename T, typename S, int NV, int WAVES, bool VEC>
-__global__ __launch_bounds__(WAVES == 8 ? 512 : 256) void block_norm_grad_kernel(BlockNormArgs p) {
-    constexpr int N = 4, LANES = 64 * WAVES, ROWS = WAVES == 1 ? 4 : 1;
-    __shared__ float lds[2 * WAVES * 2], lds1[2 * WAVES];
-    __shared__ f32x4 meet[WAVES == 1 ? 3 * NV * 64 : 1];
-    RowSum<WAVES, 1> sum1{lds1};
-    RowSum<WAVES, 2> sum2{lds};
-    const int lane = threadIdx.x % LANES;
-    f32x4 acc[3][NV];
-#pragma unroll
-    for (int k = 0; k < 3; ++k)
-#pragma unroll
-        for (int i = 0; i < NV; ++i) acc[k][i] = zero4();
-    for (long long first = (long long)blockIdx.x * ROWS; first < p.rows; first += (long long)gridDim.x * ROWS) {
-        const long long row = first + threadIdx.x / LANES;
+__global__ __launch_bounds__(RowShare<WAVES>::THREADS) void block_norm_grad_kernel(BlockNormArgs p) {
+    using Share = RowShare<WAVES>;
+    constexpr int N = 16 / sizeof(T), LANES = Share::LANES, ROWS = Share::ROWS;
+    __shared__ float lds[ROWS][2 * WAVES * 2], lds1[ROWS][2 * WAVES];
+    __shared__ float meet[ROWS > 1 ? (ROWS - 1) * NV * N * LANES : 1];
+    Share at;
+    RowSum<WAVES, 1> sum1{lds1[threadIdx.x / LANES]};
+    RowSum<WAVES, 2> sum2{lds[threadIdx.x / LANES]};
+    RowOf<T, N, NV, VEC> rx, rg, rdy;
+    RowOf<S, N, NV, VEC> rr, rdr;
+    auto request = [&](long long row) __attribute__((always_inline)) {
         const bool live = row < p.rows;
-        const int E = live ? p.E : 0;
-        float x[NV][N], r[NV][N], m[NV][N], t[NV][N];    // xhat; r, then rhat; dy; the gradient of r
+        rx.load(p.x, row, live, p.E, LANES, at.lane);
+        if (p.gate) rg.load(p.gate, row, live, p.E, LANES, at.lane);
+        else rg.clear();
+        if (p.residual) rr.load(p.residual, row, live, p.E, LANES, at.lane);
+        else rr.clear();
+        if (p.dy) rdy.load(p.dy, row, live, p.E, LANES, at.lane);
+        else rdy.clear();
+        if (p.dr) rdr.load(p.dr, row, live, p.E, LANES, at.lane);
+        else rdr.clear();
+    };
+    const int turns = at.turns(p.rows);
+    if (turns > 0) request(at.row);
+    float w[NV][N], pw[NV][N], sc[NV][N], acc[3][NV][N];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e = (i * LANES + at.lane) * N;
+        ld_vector<N, VEC>(p.weight, p.w_f32, p.E, e, 1.f, w[i]);
+        ld_vector<N, VEC>(p.post, p.p_f32, p.E, e, 1.f, pw[i]);
+        ld_vector<N, VEC>(p.scale, p.s_f32, p.E, e, p.factor, sc[i]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[k][i][j] = 0.f;
+    }
+    for (int turn = turns; turn > 0; --turn, at.row += at.step) {
+        const int E = at.row < p.rows ? p.E : 0;
+        // xhat; r; dy, then the gradient of xhat; the gradient of r; act(gate) and its derivative
+        float x[NV][N], r[NV][N], m[NV][N], t[NV][N], a[NV][N], da[NV][N];
         float inv = 1.f, s1[1] = {0.f};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int e = (i * LANES + lane) * N;
-            ld_row<T, N, VEC>(p.x, row, E, e, x[i]);
-            if (p.residual) ld_row<S, N, VEC>(p.residual, row, E, e, r[i]);
-            else
+            float g[N];
 #pragma unroll
-                for (int j = 0; j < N; ++j) r[i][j] = 0.f;
-            if (p.dy) ld_row<T, N, VEC>(p.dy, row, E, e, m[i]);
-            else
-#pragma unroll
-                for (int j = 0; j < N; ++j) m[i][j] = 0.f;
-            if (p.dr) ld_row<S, N, VEC>(p.dr, row, E, e, t[i]);
-            else
-#pragma unroll
-                for (int j = 0; j < N; ++j) t[i][j] = 0.f;
-#pragma unroll
-            for (int j = 0; j < N; ++j) s1[0] = __builtin_fmaf(x[i][j], x[i][j], s1[0]);
+            for (int j = 0; j < N; ++j) {
+                x[i][j] = rx.p[i][j];
+                r[i][j] = rr.p[i][j];
+                m[i][j] = rdy.p[i][j];
+                t[i][j] = rdr.p[i][j];
+                g[j] = rg.p[i][j];
+                a[i][j] = 1.f;
+                da[i][j] = 0.f;
+                s1[0] = __builtin_fmaf(x[i][j], x[i][j], s1[0]);
+            }
+            if (p.gate) activate<T, N>(p.act, g, a[i], da[i]);
         }
+        if (turn > 1) request(at.row + at.step);
         if (p.post_norm) {
             sum1(s1);
             inv = 1.f / sqrtf(__builtin_fmaf(s1[0], p.inv_e, p.eps));
         }
         float s2[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int e = (i * LANES + lane) * N;
-            float w[N], pw[N], sc[N], g[N], a[N], da[N];
-            ld_vector<N, VEC>(p.weight, p.w_f32, p.E, e, 1.f, w);
-            ld_vector<N, VEC>(p.post, p.p_f32, p.E, e, 1.f, pw);
-            ld_vector<N, VEC>(p.scale, p.s_f32, p.E, e, p.factor, sc);
-            if (p.gate) { ld_row<T, N, VEC>(p.gate, row, E, e, g); activate<T, N>(p.act, g, a, da); }
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 x[i][j] *= inv;
-                float u = x[i][j] * pw[j];
-                if (p.gate) u *= a[j];
-                r[i][j] = __builtin_fmaf(sc[j], u, r[i][j]);
+                r[i][j] = __builtin_fmaf(sc[i][j], x[i][j] * pw[i][j] * a[i][j], r[i][j]);
                 s2[0] = __builtin_fmaf(r[i][j], r[i][j], s2[0]);
-                s2[1] = __builtin_fmaf(m[i][j] * w[j], r[i][j], s2[1]);
+                s2[1] = __builtin_fmaf(m[i][j] * w[i][j], r[i][j], s2[1]);
             }
-        }
         sum2(s2);
         const float ir = 1.f / sqrtf(__builtin_fmaf(s2[0], p.inv_e, p.eps)), along = s2[1] * ir * p.inv_e;
         s1[0] = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int e = (i * LANES + lane) * N;
-            float w[N], pw[N], sc[N], g[N], a[N], da[N], dg[N];
-            ld_vector<N, VEC>(p.weight, p.w_f32, p.E, e, 1.f, w);
-            ld_vector<N, VEC>(p.post, p.p_f32, p.E, e, 1.f, pw);
-            ld_vector<N, VEC>(p.scale, p.s_f32, p.E, e, p.factor, sc);
-            if (p.gate) { ld_row<T, N, VEC>(p.gate, row, E, e, g); activate<T, N>(p.act, g, a, da); }
-            f32x4 dw = acc[0][i], dp = acc[1][i], ds = acc[2][i];
+            const int e = (i * LANES + at.lane) * N;
+            float dg[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const float rh = r[i][j] * ir;
-                t[i][j] = __builtin_fmaf(ir, m[i][j] * w[j] - rh * along, t[i][j]);
-                dw[j] = __builtin_fmaf(m[i][j], rh, dw[j]);
-                const float pv = x[i][j] * pw[j];
-                ds[j] = __builtin_fmaf(t[i][j], p.gate ? pv * a[j] : pv, ds[j]);
-                float du = t[i][j] * sc[j];
-                if (p.gate) { dg[j] = du * pv * da[j]; du *= a[j]; }
-                dp[j] = __builtin_fmaf(du, x[i][j], dp[j]);
-                m[i][j] = du * pw[j];
+                const float rh = r[i][j] * ir, pv = x[i][j] * pw[i][j];
+                t[i][j] = __builtin_fmaf(ir, m[i][j] * w[i][j] - rh * along, t[i][j]);
+                acc[0][i][j] = __builtin_fmaf(m[i][j], rh, acc[0][i][j]);
+                acc[2][i][j] = __builtin_fmaf(t[i][j], pv * a[i][j], acc[2][i][j]);
+                const float du = t[i][j] * sc[i][j], dp = du * a[i][j];
+                dg[j] = du * pv * da[i][j];
+                acc[1][i][j] = __builtin_fmaf(dp, x[i][j], acc[1][i][j]);
+                m[i][j] = dp * pw[i][j];
                 s1[0] = __builtin_fmaf(m[i][j], x[i][j], s1[0]);
             }
-            acc[0][i] = dw; acc[1][i] = dp; acc[2][i] = ds;
-            if (p.gate) st_row<T, N, VEC>(p.dgate, row, E, e, dg);
-            if (p.dresidual) st_row<S, N, VEC>(p.dresidual, row, E, e, t[i]);
+            if (p.gate) st_row<T, N, VEC>(p.dgate, at.row, E, e, dg);
+            if (p.dresidual) st_row<S, N, VEC>(p.dresidual, at.row, E, e, t[i]);
         }
         float back = 0.f;
         if (p.post_norm) { sum1(s1); back = s1[0] * p.inv_e; }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int e = (i * LANES + lane) * N;
+            const int e = (i * LANES + at.lane) * N;
             float d[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) d[j] = p.post_norm ? inv * (m[i][j] - x[i][j] * back) : m[i][j];
-            st_row<T, N, VEC>(p.dx, row, E, e, d);
+            st_row<T, N, VEC>(p.dx, at.row, E, e, d);
         }
     }
+    // rows that a workgroup has side by side: their sums meet in LDS
     float* const to = p.part + (long long)blockIdx.x * 3 * p.E;
+    const int mine = threadIdx.x / LANES;
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-        if constexpr (WAVES == 1) {                       // the four waves hold the same channels
-            const int wave = threadIdx.x >> 6;
+        if constexpr (ROWS > 1) {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (wave) meet[((wave - 1) * NV + i) * 64 + lane] = acc[k][i];
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (mine) meet[((mine - 1) * NV * N + i * N + j) * LANES + at.lane] = acc[k][i][j];
             __syncthreads();
+            if (mine) continue;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (!wave) acc[k][i] += (meet[i * 64 + lane] + meet[(NV + i) * 64 + lane]) + meet[(2 * NV + i) * 64 + lane];
-            if (wave) continue;
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+#pragma unroll
+                    for (int o = 0; o < ROWS - 1; ++o) acc[k][i][j] += meet[(o * NV * N + i * N + j) * LANES + at.lane];
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int e = (i * LANES + lane) * N;
-            const f32x4 v = acc[k][i];
+            const int e = (i * LANES + at.lane) * N;
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (e + j < p.E) to[k * p.E + e + j] = v[j];
+                if (e + j < p.E) to[k * p.E + e + j] = acc[k][i][j];
         }
     }
 }
 
 constexpr int BLOCK_NORM_MOST = 4096;     // a row lies in the registers of eight waves at the most
 struct BlockNormCfg { int nv, waves; bool vec; long long wgs; };
-static int block_norm_config(const hdla_block_norm_dims* d, bool bwd, BlockNormCfg& c) {
+constexpr long long BLOCK_NORM_WGS = 2048, BLOCK_NORM_GRAD_WGS = 768;
+static int block_norm_config(const hdla_block_norm_dims* d, bool bwd, BlockNormCfg& c, const void* weight = nullptr, const void* post = nullptr, const void* scale = nullptr) {
     if (!d) return HDLA_ERR_NULL;
     for (int t : {d->dtype, d->residual_dtype, d->weight_dtype, d->post_dtype, d->scale_dtype})
         if (t != HDLA_BF16 && t != HDLA_FP32) return HDLA_ERR_DTYPE;
     if (d->dtype == HDLA_FP32 && d->residual_dtype != HDLA_FP32) return HDLA_ERR_DTYPE;
     if (d->rows < 0 || d->rows > (1LL << 40) || d->E < 1 || !(d->eps >= 0.f) || d->act < ACT_NONE || d->act > ACT_SILU) return HDLA_ERR_SHAPE;
     if (d->E > BLOCK_NORM_MOST) return HDLA_ERR_SHAPE;
-    const int n = bwd || d->dtype == HDLA_FP32 ? 4 : 8, pieces = (d->E + n - 1) / n;
-    c.waves = pieces <= 64 ? 1 : pieces <= 512 ? 4 : 8;
-    c.nv = 1;
-    while (c.nv * 64 * c.waves < pieces) c.nv *= 2;
-    const long long per = c.waves == 1 ? 4 : 1, need = (d->rows + per - 1) / per;
-    c.wgs = std::max(1LL, std::min(need, bwd ? 1024LL : 4096LL));
+    const int n = d->dtype == HDLA_BF16 ? 8 : 4, pieces = (d->E + n - 1) / n;
+    c.waves = pieces <= 64 ? 1 : pieces <= 128 ? 2 : pieces <= 256 || (pieces <= 512 && n == 4) ? 4 : 8;
+    c.nv = pieces > 64 * c.waves ? 2 : 1;
+    const long long per = c.waves >= 4 ? 1 : 4 / c.waves, need = (d->rows + per - 1) / per, most = bwd ? BLOCK_NORM_GRAD_WGS : BLOCK_NORM_WGS;
+    // as many as are resident, with as many rows each as the others
+    const long long turns = (need + most - 1) / most;
+    c.wgs = std::max(1LL, turns ? (need + turns - 1) / turns : 1);
     c.vec = d->E % n == 0;
+    for (const void* q : {weight, post, scale}) c.vec = c.vec && fits(q, 16);
     return HDLA_OK;
 }
 static BlockNormArgs block_norm_args(const hdla_block_norm_dims* d) {
@@ -299,7 +354,7 @@ static BlockNormArgs block_norm_args(const hdla_block_norm_dims* d) {
     return a;
 }
 template <typename T, typename S, int NV, int WAVES> static void launch_norm_of(const BlockNormArgs& a, const BlockNormCfg& c, bool bwd, hipStream_t s) {
-    const dim3 grid((unsigned)c.wgs), block(WAVES == 8 ? 512 : 256);
+    const dim3 grid((unsigned)c.wgs), block(RowShare<WAVES>::THREADS);
     if (bwd) {
         if (c.vec) hipLaunchKernelGGL((block_norm_grad_kernel<T, S, NV, WAVES, true>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((block_norm_grad_kernel<T, S, NV, WAVES, false>), grid, block, 0, s, a);
@@ -309,10 +364,12 @@ template <typename T, typename S, int NV, int WAVES> static void launch_norm_of(
     }
 }
 template <typename T, typename S> static hipError_t launch_block_norm(const BlockNormArgs& a, const BlockNormCfg& c, bool bwd, hipStream_t s) {
+    constexpr int WIDE = sizeof(T) == 4 ? 2 : 1;          // pieces of the widest rows
     if (c.waves == 1) launch_norm_of<T, S, 1, 1>(a, c, bwd, s);
+    else if (c.waves == 2) launch_norm_of<T, S, 1, 2>(a, c, bwd, s);
     else if (c.waves == 4 && c.nv == 1) launch_norm_of<T, S, 1, 4>(a, c, bwd, s);
-    else if (c.waves == 4) launch_norm_of<T, S, 2, 4>(a, c, bwd, s);
-    else launch_norm_of<T, S, 2, 8>(a, c, bwd, s);
+    else if (c.waves == 4) launch_norm_of<T, S, WIDE, 4>(a, c, bwd, s);
+    else launch_norm_of<T, S, WIDE, 8>(a, c, bwd, s);
     return hipGetLastError();
 }
 static hipError_t launch_any(const hdla_block_norm_dims* d, const BlockNormArgs& a, const BlockNormCfg& c, bool bwd, hipStream_t s) {
@@ -327,7 +384,7 @@ using namespace hdla;
 extern "C" int hdla_block_norm_fwd(const hdla_block_norm_dims* dims, const void* x, const void* residual, const void* weight, const void* post_weight, const void* gate,
                                    const void* scale, void* y, void* r, void* stream) {
     BlockNormCfg c;
-    const int rc = block_norm_config(dims, false, c);
+    const int rc = block_norm_config(dims, false, c, weight, post_weight, scale);
     if (rc) return rc;
     if (dims->rows == 0) return HDLA_OK;
     if (!x || !y || !r) return HDLA_ERR_NULL;
@@ -346,7 +403,7 @@ extern "C" int hdla_block_norm_bwd(const hdla_block_norm_dims* dims, const void*
                                    const void* scale, const void* dy, const void* dr, void* dx, void* dresidual, void* dweight, void* dpost_weight, void* dgate,
                                    void* dscale, void* workspace, size_t workspace_bytes, void* stream) {
     BlockNormCfg c;
-    const int rc = block_norm_config(dims, true, c);
+    const int rc = block_norm_config(dims, true, c, weight, post_weight, scale);
     if (rc) return rc;
     if ((weight && !dweight) || (post_weight && !dpost_weight) || (scale && !dscale)) return HDLA_ERR_NULL;
     if (dims->rows > 0 && (!x || !dx || (gate && !dgate))) return HDLA_ERR_NULL;
@@ -360,15 +417,12 @@ extern "C" int hdla_block_norm_bwd(const hdla_block_norm_dims* dims, const void*
     const hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t e = launch_any(dims, a, c, true, s);       // (no rows: one workgroup leaves zeros)
     if (e != hipSuccess) return (int)e;
-    const struct { void* out; bool f32; } sums[3] = {{weight ? dweight : nullptr, a.w_f32 != 0}, {post_weight ? dpost_weight : nullptr, a.p_f32 != 0}, {scale ? dscale : nullptr, a.s_f32 != 0}};
-    for (int i = 0; i < 3; ++i) {
-        if (!sums[i].out) continue;
-        ColumnSums k{};
-        k.part = a.part + (long long)i * dims->E; k.rows = c.wgs;
-        k.add(sums[i].out, sums[i].f32, dims->E);
-        k.apart = 3LL * dims->E;
-        e = launch_column_sums(k, s);
-        if (e != hipSuccess) return (int)e;
-    }
-    return HDLA_OK;
+    if (!weight && !post_weight && !scale) return HDLA_OK;
+    ColumnSums k{};
+    k.part = a.part; k.rows = c.wgs;
+    k.add(weight ? dweight : nullptr, a.w_f32, dims->E);
+    k.add(post_weight ? dpost_weight : nullptr, a.p_f32, dims->E);
+    k.add(scale ? dscale : nullptr, a.s_f32, dims->E);
+    e = launch_column_sums(k, s);
+    return e == hipSuccess ? HDLA_OK : (int)e;
 }

@@ -16,8 +16,9 @@ struct ColumnSums {
     const int64_t* cu;
     int N, T;
     long long per_token, tokens_end;
+    // the next n columns (o null: of no use)
     void add(void* o, bool is_f32, long long n) {
-        if (!o || !n) return;
+        if (!n) return;
         const long long at = results ? end[results - 1] : 0;
         out[results] = o;
         f32[results] = is_f32;

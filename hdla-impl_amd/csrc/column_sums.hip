@@ -44,6 +44,7 @@ template <int PH> __global__ __launch_bounds__(256) void column_sums_kernel(Colu
     int at = 0;
     while (at + 1 < s.results && col >= s.end[at]) ++at;
     const long long e = col - (at ? s.end[at - 1] : 0);
+    if (!s.out[at]) return;
     if (s.f32[at]) static_cast<float*>(s.out[at])[e] = sum;
     else st_elem(static_cast<bf16*>(s.out[at]) + e, sum);
 }

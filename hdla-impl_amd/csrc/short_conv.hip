@@ -537,8 +537,7 @@ extern "C" int hdla_short_conv_bwd(const hdla_conv_dims* dims, const void* x, co
     ColumnSums c{};
     c.part = a.part; c.rows = rows;
     c.add(dweight, a.w_f32, (long long)dims->D * dims->W);
-    if (bias) c.add(dbias, a.b_f32, dims->D);
-    c.apart = (long long)dims->D * (dims->W + 1);
+    c.add(bias ? dbias : nullptr, a.b_f32, dims->D);
     e = launch_column_sums(c, s);
     return e == hipSuccess ? HDLA_OK : (int)e;
 }

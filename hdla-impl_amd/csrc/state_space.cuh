@@ -49,7 +49,7 @@ struct ScanArgs {
     const void* dy;                   // [rows, D]
     const float* dht;
     void *dx, *ddt, *dz;              // [rows, D]
-    float *part_bc, *part_a, *part_d, *part_bias, *dh0;
+    float *part_bc, *part_own, *dh0;
     long long rows;
     int slots;                        // sequences at a time
 };
@@ -135,7 +135,10 @@ template <int V, bool VEC> struct Raw<float, V, VEC> {
 };
 // the first n of V results, rounded to nearest
 template <typename T, int V, bool VEC> __device__ __forceinline__ void st_values(T* p, const float (&x)[V], int n) {
-    if constexpr (VEC && V % 4 == 0) {
+    if constexpr (VEC && V == 8 && sizeof(T) == 2) {
+        const s16x4 lo = to_frag<T>(f32x4{x[0], x[1], x[2], x[3]}).v, hi = to_frag<T>(f32x4{x[4], x[5], x[6], x[7]}).v;
+        *reinterpret_cast<s16x8*>(p) = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else if constexpr (VEC && V % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < V; i += 4) st_frag(p + i, to_frag<T>(f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]}));
     } else {

@@ -285,13 +285,14 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < W; ++i) s += reinterpret_cast<const float*>(meet.E)[i * 256 + e];
-        if (there) p.part_a[((long long)slot * p.DD + L.d0 + ec) * p.S + es] = s;
+        if (there) p.part_own[(long long)slot * p.DD * (p.S + 2) + (long long)(L.d0 + ec) * p.S + es] = s;
     } else if (backwards && e < CHN && (block % p.per_group) * CHN + e < p.DD / p.G) {
         float s = 0.f, b = 0.f;
 #pragma unroll
         for (int i = 0; i < W; ++i) { s += mine[i].d[e]; b += mine[i].x[e]; }
-        p.part_d[(long long)slot * p.DD + L.d0 + e] = s;
-        p.part_bias[(long long)slot * p.DD + L.d0 + e] = b;
+        float* const to = p.part_own + (long long)slot * p.DD * (p.S + 2) + (long long)p.DD * p.S + L.d0 + e;
+        to[0] = s;
+        to[p.DD] = b;
     }
 }
 
@@ -300,17 +301,9 @@ static int grad_slots(const hdla_scan_dims* d, const ScanPlan& s) {
     const long long most = std::max(1LL, 2048LL / s.blocks);
     return (int)std::min<long long>(d->N, most);
 }
-struct GradRoom { size_t bc, a, d, bias, total; };
-static GradRoom grad_room(const hdla_scan_dims* d, const ScanPlan& s, int slots) {
-    auto up = [](size_t n) { return (n + 15) / 16 * 16; };
-    GradRoom r;
-    r.bc = 0;
-    r.a = up((size_t)s.per_group * 2 * s.rows * d->G * d->S * 4);
-    r.d = r.a + up((size_t)slots * d->D * d->S * 4);
-    r.bias = r.d + up((size_t)slots * d->D * 4);
-    r.total = r.bias + up((size_t)slots * d->D * 4);
-    return r;
-}
+// partial sums of dB and dC, [blocks of a group][2][rows][G][S], and behind them those of dA, dD and d bias, [slots][D S + 2 D]
+static size_t bc_bytes(const hdla_scan_dims* d, const ScanPlan& s) { return ((size_t)s.per_group * 2 * s.rows * d->G * d->S * 4 + 15) / 16 * 16; }
+static size_t grad_bytes(const hdla_scan_dims* d, const ScanPlan& s, int slots) { return bc_bytes(d, s) + (size_t)slots * d->D * (d->S + 2) * 4; }
 template <typename T, int LPC> static void launch_grad(const ScanArgs& a, bool vec, hipStream_t s) {
     constexpr int TOK = SS_TOK, W = 8;
     const dim3 grid((unsigned)((long long)a.blocks * a.slots)), block(64 * W);
@@ -334,7 +327,7 @@ using namespace hdla;
 
 extern "C" size_t hdla_scan_workspace_bytes(const hdla_scan_dims* dims) {
     ScanPlan s;
-    return scan_plan(dims, s) ? 0 : grad_room(dims, s, grad_slots(dims, s)).total;
+    return scan_plan(dims, s) ? 0 : grad_bytes(dims, s, grad_slots(dims, s));
 }
 extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const void* dt, const void* A, const void* B, const void* C, const void* D, const void* z,
                              const void* dt_bias, const void* dy, const float* dht, const void* states, size_t states_bytes, void* dx, void* ddt, void* dA, void* dB,
@@ -347,17 +340,14 @@ extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const vo
     for (const void* q : {dy, (const void*)dht, states, (const void*)dx, (const void*)ddt, (const void*)dB, (const void*)dC, (const void*)dz, (const void*)dh0})
         if (!fits(q, 16)) return HDLA_ERR_ALIGN;
     s.slots = grad_slots(dims, s);
-    const GradRoom room = grad_room(dims, s, s.slots);
-    if (!workspace || !fits(workspace, 16) || workspace_bytes < room.total) return HDLA_ERR_WORKSPACE;
+    if (!workspace || !fits(workspace, 16) || workspace_bytes < grad_bytes(dims, s, s.slots)) return HDLA_ERR_WORKSPACE;
     if (s.rows > 0 && states_bytes < (size_t)s.ckpt * s.blocks * 1024) return HDLA_ERR_WORKSPACE;
     ScanArgs a = scan_args(dims, s, x, dt, A, B, C, D, z, dt_bias);
     a.dy = dy; a.dht = dht; a.ckpt = static_cast<float*>(const_cast<void*>(states));
     a.dx = dx; a.ddt = ddt; a.dz = dz; a.dh0 = dh0;
     char* const base = static_cast<char*>(workspace);
-    a.part_bc = reinterpret_cast<float*>(base + room.bc);
-    a.part_a = reinterpret_cast<float*>(base + room.a);
-    a.part_d = reinterpret_cast<float*>(base + room.d);
-    a.part_bias = reinterpret_cast<float*>(base + room.bias);
+    a.part_bc = reinterpret_cast<float*>(base);
+    a.part_own = reinterpret_cast<float*>(base + bc_bytes(dims, s));
     s.vec = scan_vec(dims, s, a);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const int es = dims->dtype == HDLA_BF16 ? 2 : 4;
@@ -377,15 +367,11 @@ extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const vo
     c.add(dC, es == 4, s.rows * inner);
     e = launch_column_sums(c, st);
     if (e != hipSuccess) return (int)e;
-    const struct { const float* part; void* out; int f32; long long n; } sums[3] = {
-        {a.part_a, dA, a.A_f32, (long long)dims->D * dims->S}, {a.part_d, dD, a.D_f32, dims->D}, {a.part_bias, ddt_bias, a.bias_f32, dims->D}};
-    for (const auto& q : sums) {
-        if (!q.out) continue;
-        ColumnSums k{};
-        k.part = q.part; k.rows = s.slots;
-        k.add(q.out, q.f32, q.n);
-        e = launch_column_sums(k, st);
-        if (e != hipSuccess) return (int)e;
-    }
-    return HDLA_OK;
+    ColumnSums k{};
+    k.part = a.part_own; k.rows = s.slots;
+    k.add(dA, a.A_f32, (long long)dims->D * dims->S);
+    k.add(D ? dD : nullptr, a.D_f32, dims->D);
+    k.add(dt_bias ? ddt_bias : nullptr, a.bias_f32, dims->D);
+    e = launch_column_sums(k, st);
+    return e == hipSuccess ? HDLA_OK : (int)e;
 }
