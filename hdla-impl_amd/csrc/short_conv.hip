@@ -105,68 +105,87 @@ template <typename T, int W, int V> __device__ __forceinline__ void conv_last(co
     st_values<T, V, (V > 1)>(static_cast<T*>(p.last) + (n * (W - 1) + i) * p.D + col, f, V);
 }
 
-template <typename T, int W, int V, int RUN>
-__global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs p) {
+// The taps of tokens: rows of x as they come from memory, `before` the W - 1 in front of those in `now`
+template <int W, int STEP, typename R> __device__ __forceinline__ const R& tap(const R (&before)[W - 1], const R (&now)[STEP], int i) {
+    return i < W - 1 ? before[i < W - 1 ? i : 0] : now[i >= W - 1 ? i - (W - 1) : 0];
+}
+template <typename T, int W, int V, int STEP, bool PACKED>
+__global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs p, int steps) {
+    using R = Raw<T, V, (V > 1)>;
     const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
     if (id >= p.threads) { if (p.last) conv_last<T, W, V>(p, id - p.threads); return; }
     const int col = (int)(id % p.cols) * V;
     const long long r = id / p.cols;
-    const int n = p.cu ? 0 : (int)(r / p.runs);
-    const int64_t t0 = (r - (long long)n * p.runs) * RUN;
-    const int tokens = (int)min((int64_t)RUN, p.T - t0);
+    const int n = PACKED ? 0 : (int)(r / p.runs);
+    int64_t t0 = (r - (long long)n * p.runs) * steps * STEP;
+    // (rows behind the last, asked for with a step of others, are the last one once more)
+    const T* const x0 = static_cast<const T*>(p.x.p) + n * p.x.batch + col;
+    auto row = [&](int64_t t, R& to) __attribute__((always_inline)) { to.load(x0 + min(t, (int64_t)p.T - 1) * p.x.row, V); };
+    R before[W - 1], now[STEP], next[STEP];
+#pragma unroll
+    for (int i = 0; i < STEP; ++i) row(t0 + i, now[i]);
     float w[V][W], b[V];
     ld_taps<W, V>(p.weight, p.w_f32, (long long)col * W, w, true);
 #pragma unroll
     for (int k = 0; k < V; ++k) b[k] = p.bias ? ld_param(p.bias, p.b_f32, col + k) : 0.f;
-    Where s{n, 0, p.T};
-    if (p.cu) s.find(p, t0);
-    Raw<T, V, (V > 1)> x[RUN + W - 1];
-    // (rows before the first of the batch, or of another sequence: looked at below)
+    // (before a packed batch's first token nothing is read: these rows are of another sequence, or of none)
 #pragma unroll
-    for (int i = 0; i < RUN + W - 1; ++i) {
+    for (int i = 0; i < W - 1; ++i) {
         const int64_t t = t0 - (W - 1) + i;
-        if (p.cu ? (t >= 0 && t < p.T) : t < p.T) x[i] = p.cu ? ConvRow<T, W, V>::get(p, 0, 0, t, col) : ConvRow<T, W, V>::get(p, n, 0, t, col);
-        else x[i].clear();
+        before[i] = PACKED ? ConvRow<T, W, V>::get(p, 0, 0, max(t, (int64_t)0), col) : ConvRow<T, W, V>::get(p, n, 0, t, col);
     }
-    T* const y0 = static_cast<T*>(p.y) + ((long long)n * p.T + t0) * p.D + col;
+    Where s{n, 0, p.T};
+    if (PACKED) s.find(p, t0);
+    T* y = static_cast<T*>(p.y) + ((long long)n * p.T + t0) * p.D + col;
+    for (int step = 0; step < steps && t0 < p.T; ++step, t0 += STEP) {
+        if (step + 1 < steps) {
 #pragma unroll
-    for (int i = 0; i < RUN; ++i) {
-        if (i < tokens) {
-            const int64_t t = t0 + i;
-            float f[V];
-#pragma unroll
-            for (int k = 0; k < V; ++k) f[k] = b[k];
-            bool none = false, early = false;
-            if (p.cu) {
-                if (i && t >= s.eos) s.next(p, t);
-                none = t < s.bos;
-                early = t - s.bos < W - 1;
-            }
-            if (!early) {
-#pragma unroll
-                for (int j = 0; j < W; ++j)
-#pragma unroll
-                    for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(w[k][j], x[i + j][k], f[k]);
-            } else if (!none) {
-#pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    const Raw<T, V, (V > 1)> e = ConvRow<T, W, V>::get(p, s.n, s.bos, t - s.bos - (W - 1) + j, col);
-#pragma unroll
-                    for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(w[k][j], e[k], f[k]);
-                }
-            }
-            if (p.silu) {
-                float g[V];
-                sigmoid_each<T, V>(f, g);
-#pragma unroll
-                for (int k = 0; k < V; ++k) f[k] *= g[k];
-            }
-            if (none) {
-#pragma unroll
-                for (int k = 0; k < V; ++k) f[k] = 0.f;
-            }
-            st_values<T, V, (V > 1)>(y0 + (long long)i * p.D, f, V);
+            for (int i = 0; i < STEP; ++i) row(t0 + STEP + i, next[i]);
         }
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) {
+            const int64_t t = t0 + i;
+            if (t < p.T) {
+                float f[V];
+#pragma unroll
+                for (int k = 0; k < V; ++k) f[k] = b[k];
+                bool none = false, early = false;
+                if (PACKED) {
+                    if (t >= s.eos) s.next(p, t);
+                    none = t < s.bos;
+                    early = t - s.bos < W - 1;
+                }
+                if (!early) {
+#pragma unroll
+                    for (int j = 0; j < W; ++j)
+#pragma unroll
+                        for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(w[k][j], tap<W, STEP>(before, now, i + j)[k], f[k]);
+                } else if (!none) {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) {
+                        const R e = ConvRow<T, W, V>::get(p, s.n, s.bos, t - s.bos - (W - 1) + j, col);
+#pragma unroll
+                        for (int k = 0; k < V; ++k) f[k] = __builtin_fmaf(w[k][j], e[k], f[k]);
+                    }
+                }
+                if (p.silu) {
+                    float g[V];
+                    sigmoid_each<T, V>(f, g);
+#pragma unroll
+                    for (int k = 0; k < V; ++k) f[k] *= g[k];
+                }
+                if (none) {
+#pragma unroll
+                    for (int k = 0; k < V; ++k) f[k] = 0.f;
+                }
+                st_values<T, V, (V > 1)>(y, f, V);
+            }
+            y += p.D;
+        }
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i) before[i] = now[STEP - (W - 1) + i];
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) now[i] = next[i];
     }
 }
 
@@ -233,9 +252,11 @@ template <typename T, int W, int V> __device__ __forceinline__ void conv_dstate(
     st_values<T, V, (V > 1)>(static_cast<T*>(p.dstate) + (n * (W - 1) + i) * p.D + col, d, V);
 }
 
-// A workgroup is 64 columns (fewer where there are fewer) x 4 runs of RUNS x STEP tokens: their sums of dw and dbias meet in LDS.
-template <typename T, int W, int V, int STEP>
+// A workgroup is 64 columns (fewer where there are fewer) x 4 runs of steps x STEP tokens: their sums of dw and dbias meet in LDS.  A run walks its tokens and the
+// W - 1 behind them: g_t from its taps, then dx_{t-W+1}, which by then has all the g that it needs.
+template <typename T, int W, int V, int STEP, bool PACKED>
 __global__ __launch_bounds__(256) void short_conv_grad_kernel(ConvArgs p, int steps, long long col_blocks, long long row_blocks) {
+    using R = Raw<T, V, (V > 1)>;
     __shared__ float red[3][V * (W + 1)][64];
     if (blockIdx.x >= col_blocks * row_blocks) {
         if (p.dstate) conv_dstate<T, W, V>(p, (blockIdx.x - col_blocks * row_blocks) * 256 + threadIdx.x);
@@ -243,9 +264,9 @@ __global__ __launch_bounds__(256) void short_conv_grad_kernel(ConvArgs p, int st
     }
     const int c = (int)(blockIdx.x % col_blocks) * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
     const long long r = blockIdx.x / col_blocks * 4 + wave;
-    const bool live = c < p.cols && r < (long long)(p.cu ? 1 : p.N) * p.runs;
-    const int col = c * V, n = p.cu || !live ? 0 : (int)(r / p.runs);
+    const int col = c * V, n = PACKED ? 0 : (int)(r / p.runs);
     const int64_t first = (r - (long long)n * p.runs) * steps * STEP;
+    const bool live = c < p.cols && r < (long long)(PACKED ? 1 : p.N) * p.runs && first < p.T;
     float dw[V][W], db[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
@@ -254,101 +275,108 @@ __global__ __launch_bounds__(256) void short_conv_grad_kernel(ConvArgs p, int st
         for (int j = 0; j < W; ++j) dw[k][j] = 0.f;
     }
     if (live) {
-        float w[V][W], b[V];
+        const int64_t end = min(first + (int64_t)steps * STEP, (int64_t)p.T);          // of this run's own tokens
+        const T *const x0 = static_cast<const T*>(p.x.p) + n * p.x.batch + col, *const dy0 = static_cast<const T*>(p.dy) + (long long)n * p.T * p.D + col;
+        T* const dx0 = static_cast<T*>(p.dx) + (long long)n * p.T * p.D + col;
+        // (rows behind the last, asked for with a step of others, are the last one once more)
+        auto rows = [&](int64_t t, R& x, R& dy) __attribute__((always_inline)) {
+            const int64_t at = min(t, (int64_t)p.T - 1);
+            x.load(x0 + at * p.x.row, V);
+            dy.load(dy0 + at * p.D, V);
+        };
+        R before[W - 1], x[STEP], dy[STEP], xn[STEP], dyn[STEP];
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) rows(first + i, x[i], dy[i]);
+        float w[V][W], b[V], ring[W][V];                  // ring: g of the last W tokens
         ld_taps<W, V>(p.weight, p.w_f32, (long long)col * W, w, true);
 #pragma unroll
-        for (int k = 0; k < V; ++k) b[k] = p.bias ? ld_param(p.bias, p.b_f32, col + k) : 0.f;
-        const long long row0 = (long long)n * p.T;
-        const T* const dy0 = static_cast<const T*>(p.dy) + row0 * p.D + col;
-        T* const dx0 = static_cast<T*>(p.dx) + row0 * p.D + col;
-        Where s{n, 0, p.T};
-        if (p.cu) s.find(p, first);
-        for (int step = 0; step < steps; ++step) {
-            const int64_t t0 = first + (int64_t)step * STEP;
-            const int tokens = (int)min((int64_t)STEP, p.T - t0);
-            if (tokens <= 0) break;
-            // g_t of this step's tokens and of the W - 1 behind them, x from W - 1 before
-            Raw<T, V, (V > 1)> x[STEP + 2 * (W - 1)], dy[STEP + W - 1];
+        for (int k = 0; k < V; ++k) {
+            b[k] = p.bias ? ld_param(p.bias, p.b_f32, col + k) : 0.f;
 #pragma unroll
-            for (int i = 0; i < STEP + 2 * (W - 1); ++i) {
-                const int64_t t = t0 - (W - 1) + i;
-                if (p.cu ? (t >= 0 && t < p.T) : t < p.T) x[i] = ConvRow<T, W, V>::get(p, n, 0, t, col);
-                else x[i].clear();
+            for (int j = 0; j < W; ++j) ring[j][k] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i) {
+            const int64_t t = first - (W - 1) + i;
+            before[i] = PACKED ? ConvRow<T, W, V>::get(p, 0, 0, max(t, (int64_t)0), col) : ConvRow<T, W, V>::get(p, n, 0, t, col);
+        }
+        Where q{n, 0, p.T}, s{n, 0, p.T};                 // of the token whose g is formed; of the one whose dx is
+        if (PACKED) { q.find(p, first); s = q; }
+        for (int64_t t0 = first; t0 < end + (W - 1); t0 += STEP) {
+            if (t0 + STEP < end + (W - 1)) {
+#pragma unroll
+                for (int i = 0; i < STEP; ++i) rows(t0 + STEP + i, xn[i], dyn[i]);
             }
 #pragma unroll
-            for (int i = 0; i < STEP + W - 1; ++i) {
-                dy[i].clear();
-                if (t0 + i < p.T) dy[i].load(dy0 + (t0 + i) * p.D, V);
-            }
-            float ring[W][V];                             // g of the last W tokens
-            Where q = s;
-#pragma unroll
-            for (int i = 0; i < STEP + W - 1; ++i) {
-                const int64_t t = t0 + i;
-                float g[V], xf[W][V];
+            for (int i = 0; i < STEP; ++i) {
+                const int64_t t = t0 + i, to = t - (W - 1);
+                float g[V];
 #pragma unroll
                 for (int k = 0; k < V; ++k) g[k] = 0.f;
-                bool none = t >= p.T, early = false;
-                if (p.cu && !none) {
+                bool none = t >= p.T || t >= end + (W - 1), early = false;
+                if (PACKED && !none) {
                     if (t >= q.eos) q.next(p, t);
                     none = t < q.bos;
                     early = t - q.bos < W - 1;
                 }
+                if (!none) {
+                    float xf[W][V];
 #pragma unroll
-                for (int j = 0; j < W; ++j)
+                    for (int j = 0; j < W; ++j)
 #pragma unroll
-                    for (int k = 0; k < V; ++k) xf[j][k] = x[i + j][k];
-                if (early && !none) {
+                        for (int k = 0; k < V; ++k) xf[j][k] = tap<W, STEP>(before, x, i + j)[k];
+                    if (PACKED && early) {
 #pragma unroll
-                    for (int j = 0; j < W; ++j) {
-                        const Raw<T, V, (V > 1)> e = ConvRow<T, W, V>::get(p, q.n, q.bos, t - q.bos - (W - 1) + j, col);
+                        for (int j = 0; j < W; ++j) {
+                            const R e = ConvRow<T, W, V>::get(p, q.n, q.bos, t - q.bos - (W - 1) + j, col);
 #pragma unroll
-                        for (int k = 0; k < V; ++k) xf[j][k] = e[k];
-                    }
-                }
-                if (!none) conv_g<T, W, V>(p, w, b, xf, dy[i], g);
-                if (i < STEP && !none) {
-#pragma unroll
-                    for (int k = 0; k < V; ++k) {
-                        db[k] += g[k];
-#pragma unroll
-                        for (int j = 0; j < W; ++j) dw[k][j] = __builtin_fmaf(g[k], xf[j][k], dw[k][j]);
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < V; ++k) ring[i % W][k] = g[k];
-                // token t - (W - 1) has all it needs: g of itself to t, as far as they are of its sequence
-                if (i >= W - 1) {
-                    const int64_t to = t - (W - 1);
-                    if (to < p.T && i - (W - 1) < tokens) {
-                        Where o = s;
-                        if (p.cu) {
-                            if (to >= s.eos) s.next(p, to);
-                            o = s;
+                            for (int k = 0; k < V; ++k) xf[j][k] = e[k];
                         }
-                        float d[V];
+                    }
+                    conv_g<T, W, V>(p, w, b, xf, dy[i], g);
+                    if (t < end) {
+#pragma unroll
+                        for (int k = 0; k < V; ++k) {
+                            db[k] += g[k];
+#pragma unroll
+                            for (int j = 0; j < W; ++j) dw[k][j] = __builtin_fmaf(g[k], xf[j][k], dw[k][j]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) ring[j][k] = ring[j + 1][k];
+#pragma unroll
+                for (int k = 0; k < V; ++k) ring[W - 1][k] = g[k];
+                if (to >= first && to < end) {
+                    if (PACKED && to >= s.eos) s.next(p, to);
+                    float d[V];
+#pragma unroll
+                    for (int k = 0; k < V; ++k) d[k] = 0.f;
+#pragma unroll
+                    for (int m = 0; m < W; ++m) {         // g_{to + m} through tap W - 1 - m (none behind the last token: g is zero there)
+                        if (!PACKED || to + m < s.eos) {
+#pragma unroll
+                            for (int k = 0; k < V; ++k) d[k] = __builtin_fmaf(w[k][W - 1 - m], ring[m][k], d[k]);
+                        }
+                    }
+                    if (PACKED && to < s.bos) {
 #pragma unroll
                         for (int k = 0; k < V; ++k) d[k] = 0.f;
+                    } else if (p.dlast && s.eos - to <= W - 1) {
+                        R e;
+                        e.load(static_cast<const T*>(p.dlast) + ((long long)s.n * (W - 1) + (W - 1 - (s.eos - to))) * p.D + col, V);
 #pragma unroll
-                        for (int m = 0; m < W; ++m) {     // g_{to + m} through tap W - 1 - m
-                            const bool mine = to + m < o.eos;
-#pragma unroll
-                            for (int k = 0; k < V; ++k)
-                                if (mine) d[k] = __builtin_fmaf(w[k][W - 1 - m], ring[(i + 1 + m) % W][k], d[k]);
-                        }
-                        if (p.cu && to < o.bos) {
-#pragma unroll
-                            for (int k = 0; k < V; ++k) d[k] = 0.f;
-                        } else if (p.dlast && o.eos - to <= W - 1) {
-                            Raw<T, V, (V > 1)> e;
-                            e.load(static_cast<const T*>(p.dlast) + ((long long)o.n * (W - 1) + (W - 1 - (o.eos - to))) * p.D + col, V);
-#pragma unroll
-                            for (int k = 0; k < V; ++k) d[k] += e[k];
-                        }
-                        st_values<T, V, (V > 1)>(dx0 + to * p.D, d, V);
+                        for (int k = 0; k < V; ++k) d[k] += e[k];
                     }
+                    st_values<T, V, (V > 1)>(dx0 + to * p.D, d, V);
                 }
             }
+#pragma unroll
+            for (int i = 0; i < W - 1; ++i) before[i] = x[STEP - (W - 1) + i];
+#pragma unroll
+            for (int i = 0; i < STEP; ++i) { x[i] = xn[i]; dy[i] = dyn[i]; }
         }
     }
     if (wave) {
@@ -410,7 +438,12 @@ __global__ __launch_bounds__(256) void short_conv_step_kernel(ConvArgs p) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-constexpr int CONV_RUN = 16, CONV_STEP = 8, CONV_STEPS = 4;
+constexpr int CONV_STEP = 8;
+// Steps of a run: the more, the fewer tokens are read twice; as many runs as give every compute unit `waves` waves
+static int conv_steps(long long rows, long long cols, int T, int waves, int most) {
+    const long long threads = waves * 64LL * 256, steps = rows * cols / (threads * CONV_STEP);
+    return (int)std::max(1LL, std::min<long long>({steps, (long long)most, (T + CONV_STEP - 1) / CONV_STEP}));
+}
 static int conv_check(const hdla_conv_dims* d) {
     if (!d) return HDLA_ERR_NULL;
     for (int t : {d->dtype, d->weight_dtype, d->bias_dtype})
@@ -437,14 +470,19 @@ static ConvArgs conv_args(const hdla_conv_dims* d, const void* x, const void* we
 #define HDLA_CONV_WIDTHS(CASE) CASE(2) CASE(3) CASE(4)
 
 template <typename T, int V> static hipError_t launch_conv(ConvArgs a, int W, hipStream_t s) {
-    a.cols = (a.D + V - 1) / V;
-    a.runs = (a.T + CONV_RUN - 1) / CONV_RUN;
+    a.cols = a.D / V;
+    const int steps = conv_steps((long long)a.T * (a.cu ? 1 : a.N), a.cols, a.T, 8, 8);
+    a.runs = (a.T + steps * CONV_STEP - 1) / (steps * CONV_STEP);
     a.threads = (long long)a.cols * a.runs * (a.cu ? 1 : a.N);
     const long long all = a.threads + (a.last ? (long long)a.cols * (W - 1) * a.N : 0), blocks = (all + 255) / 256;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
     if (!blocks) return hipSuccess;
     switch (W) {
-#define HDLA_CASE(WW) case WW: hipLaunchKernelGGL((short_conv_kernel<T, WW, V, CONV_RUN>), dim3((unsigned)blocks), dim3(256), 0, s, a); break;
+#define HDLA_CASE(WW)                                                                                                                            \
+    case WW:                                                                                                                                     \
+        if (a.cu) hipLaunchKernelGGL((short_conv_kernel<T, WW, V, CONV_STEP, true>), dim3((unsigned)blocks), dim3(256), 0, s, a, steps);         \
+        else hipLaunchKernelGGL((short_conv_kernel<T, WW, V, CONV_STEP, false>), dim3((unsigned)blocks), dim3(256), 0, s, a, steps);             \
+        break;
         HDLA_CONV_WIDTHS(HDLA_CASE)
 #undef HDLA_CASE
     }
@@ -462,17 +500,27 @@ template <typename T, int V> static hipError_t launch_conv_step(ConvArgs a, int 
     }
     return hipGetLastError();
 }
-// runs of the backward pass, and the rows of partial sums that they leave: four runs a row
-static long long grad_runs(const hdla_conv_dims* d) { return (d->T + CONV_STEP * CONV_STEPS - 1) / (CONV_STEP * CONV_STEPS); }
-static long long grad_rows(const hdla_conv_dims* d) { return (grad_runs(d) * (d->cu_seqlens ? 1 : d->N) + 3) / 4; }
-template <typename T, int V> static hipError_t launch_conv_grad(ConvArgs a, int W, long long runs, long long rows, hipStream_t s) {
+// Steps of a run of the backward pass, its runs, and the rows of partial sums that they leave: four runs a row
+struct ConvGradPlan { int steps; long long runs, rows; };
+static ConvGradPlan conv_grad_plan(const hdla_conv_dims* d) {
+    ConvGradPlan g;
+    g.steps = conv_steps((long long)d->T * d->B, (d->D + 3) / 4, d->T, 6, 8);
+    g.runs = (d->T + g.steps * CONV_STEP - 1) / (g.steps * CONV_STEP);
+    g.rows = (g.runs * (d->cu_seqlens ? 1 : d->N) + 3) / 4;
+    return g;
+}
+template <typename T, int V> static hipError_t launch_conv_grad(ConvArgs a, int W, const ConvGradPlan& g, hipStream_t s) {
     a.cols = a.D / V;
-    a.runs = (int)runs;
-    const long long col_blocks = (a.cols + 63) / 64, states = a.dstate ? ((long long)a.cols * (W - 1) * a.N + 255) / 256 : 0, blocks = col_blocks * rows + states;
+    a.runs = (int)g.runs;
+    const long long col_blocks = (a.cols + 63) / 64, states = a.dstate ? ((long long)a.cols * (W - 1) * a.N + 255) / 256 : 0, blocks = col_blocks * g.rows + states;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
     if (!blocks) return hipSuccess;
     switch (W) {
-#define HDLA_CASE(WW) case WW: hipLaunchKernelGGL((short_conv_grad_kernel<T, WW, V, CONV_STEP>), dim3((unsigned)blocks), dim3(256), 0, s, a, CONV_STEPS, col_blocks, rows); break;
+#define HDLA_CASE(WW)                                                                                                                                                  \
+    case WW:                                                                                                                                                           \
+        if (a.cu) hipLaunchKernelGGL((short_conv_grad_kernel<T, WW, V, CONV_STEP, true>), dim3((unsigned)blocks), dim3(256), 0, s, a, g.steps, col_blocks, g.rows);    \
+        else hipLaunchKernelGGL((short_conv_grad_kernel<T, WW, V, CONV_STEP, false>), dim3((unsigned)blocks), dim3(256), 0, s, a, g.steps, col_blocks, g.rows);        \
+        break;
         HDLA_CONV_WIDTHS(HDLA_CASE)
 #undef HDLA_CASE
     }
@@ -515,7 +563,7 @@ extern "C" int hdla_short_conv_step(const hdla_conv_dims* dims, const void* x, c
     return e == hipSuccess ? HDLA_OK : (int)e;
 }
 extern "C" size_t hdla_short_conv_workspace_bytes(const hdla_conv_dims* dims) {
-    return conv_check(dims) ? 0 : std::max<size_t>((size_t)grad_rows(dims) * dims->D * (dims->W + 1) * 4, 16);
+    return conv_check(dims) ? 0 : std::max<size_t>((size_t)conv_grad_plan(dims).rows * dims->D * (dims->W + 1) * 4, 16);
 }
 extern "C" int hdla_short_conv_bwd(const hdla_conv_dims* dims, const void* x, const void* weight, const void* bias, const void* state, const void* dy, const void* dlast,
                                    void* dx, void* dweight, void* dbias, void* dstate, void* workspace, size_t workspace_bytes, void* stream) {
@@ -529,13 +577,13 @@ extern "C" int hdla_short_conv_bwd(const hdla_conv_dims* dims, const void* x, co
     a.dy = dy; a.dlast = dlast; a.dx = dx; a.dstate = dstate;
     a.part = static_cast<float*>(workspace);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const long long runs = grad_runs(dims), rows = grad_rows(dims);
+    const ConvGradPlan g = conv_grad_plan(dims);
     hipError_t e;
-    if (dims->dtype == HDLA_BF16) e = conv_vec(dims, 4, a) ? launch_conv_grad<bf16, 4>(a, dims->W, runs, rows, s) : launch_conv_grad<bf16, 1>(a, dims->W, runs, rows, s);
-    else e = conv_vec(dims, 4, a) ? launch_conv_grad<float, 4>(a, dims->W, runs, rows, s) : launch_conv_grad<float, 1>(a, dims->W, runs, rows, s);
+    if (dims->dtype == HDLA_BF16) e = conv_vec(dims, 4, a) ? launch_conv_grad<bf16, 4>(a, dims->W, g, s) : launch_conv_grad<bf16, 1>(a, dims->W, g, s);
+    else e = conv_vec(dims, 4, a) ? launch_conv_grad<float, 4>(a, dims->W, g, s) : launch_conv_grad<float, 1>(a, dims->W, g, s);
     if (e != hipSuccess) return (int)e;
     ColumnSums c{};
-    c.part = a.part; c.rows = rows;
+    c.part = a.part; c.rows = g.rows;
     c.add(dweight, a.w_f32, (long long)dims->D * dims->W);
     c.add(bias ? dbias : nullptr, a.b_f32, dims->D);
     e = launch_column_sums(c, s);
