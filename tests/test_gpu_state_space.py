@@ -266,7 +266,7 @@ def test_another_stream_and_two_calls_at_once():
 
 # ---- one token -------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("nb,d,S,G", [(1, 16, 16, 1), (3, 5, 3, 1), (2, 64, 8, 2), (7, 33, 12, 3), (1, 7, 64, 1), (2, 24, 20, 2)])
+@pytest.mark.parametrize("nb,d,S,G", [(1, 16, 16, 1), (3, 5, 3, 1), (2, 64, 8, 2), (7, 33, 12, 3), (1, 7, 64, 1), (2, 24, 20, 2), (61, 2048, 16, 1), (258, 520, 15, 2)])
 def test_step(nb, d, S, G, dtype):
     low, ref, _, _ = make(nb * 10 + d, nb, 1, d, S, G, dtype)
     v = put(low, False)
