@@ -58,7 +58,7 @@ struct Api {
     HDLA_FN(normalize_bwd_later); HDLA_FN(layer_up_wgrad_later); HDLA_FN(run_sums);
     HDLA_FN(layer_step); HDLA_FN(rows_gemm_norm);
     HDLA_FN(short_conv_fwd); HDLA_FN(short_conv_workspace_bytes); HDLA_FN(short_conv_bwd); HDLA_FN(short_conv_step);
-    HDLA_FN(scan_states_bytes); HDLA_FN(scan_fwd); HDLA_FN(scan_workspace_bytes); HDLA_FN(scan_bwd); HDLA_FN(scan_step);
+    HDLA_FN(scan_states_bytes); HDLA_FN(scan_fwd); HDLA_FN(scan_fwd_workspace_bytes); HDLA_FN(scan_workspace_bytes); HDLA_FN(scan_bwd); HDLA_FN(scan_step);
     HDLA_FN(block_norm_fwd); HDLA_FN(block_norm_workspace_bytes); HDLA_FN(block_norm_bwd);
 #undef HDLA_FN
 } api;
@@ -1231,7 +1231,7 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HDLA_FN(normalize_bwd_later) HDLA_FN(layer_up_wgrad_later) HDLA_FN(run_sums)
     HDLA_FN(rows_gemm_norm)
     HDLA_FN(short_conv_fwd) HDLA_FN(short_conv_workspace_bytes) HDLA_FN(short_conv_bwd) HDLA_FN(short_conv_step)
-    HDLA_FN(scan_states_bytes) HDLA_FN(scan_fwd) HDLA_FN(scan_workspace_bytes) HDLA_FN(scan_bwd) HDLA_FN(scan_step)
+    HDLA_FN(scan_states_bytes) HDLA_FN(scan_fwd) HDLA_FN(scan_fwd_workspace_bytes) HDLA_FN(scan_workspace_bytes) HDLA_FN(scan_bwd) HDLA_FN(scan_step)
     HDLA_FN(block_norm_fwd) HDLA_FN(block_norm_workspace_bytes) HDLA_FN(block_norm_bwd)
 #undef HDLA_FN
     Py_INCREF(a[1]);

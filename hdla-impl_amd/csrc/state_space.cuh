@@ -51,8 +51,12 @@ struct ScanArgs {
     void *dx, *ddt, *dz;              // [rows, D]
     float *part_bc, *part_own, *dh0;
     long long rows;
-    int slots;                        // sequences at a time
+    int slots;                        // units (sequences, or segments of them) at a time
+    // segments: 0, or how many tokens one has; `units` of them, and for each [blocks][256] what it leaves if nothing enters, and [blocks][256] its decays
+    int seg, units;
+    float* ends;
 };
+constexpr int SS_SEGMENT = 128;       // segments are multiples of it
 
 // V elements of T as they come from memory; VEC: with loads of several, else (rows at any address) one by one
 template <typename T, int V, bool VEC> struct Raw;
@@ -192,10 +196,23 @@ template <typename T, int N> __device__ __forceinline__ void sigmoid_each(const 
 
 constexpr float LN2 = 0.69314718055994530942f;
 
-// Consecutive blocks of channels share cache lines: they go to workgroups of one XCD (which take the workgroups in turns).
-__device__ __forceinline__ int xcd_share(int id, int total) {
-    const int xcd = id & 7, q = total >> 3, r = total & 7;
-    return xcd * q + min(xcd, r) + (id >> 3);
+// Which unit and block of channels a workgroup has.  Workgroups go to the eight XCDs in turns, and neighbouring blocks share cache lines: each XCD has an eighth of the
+// blocks, of all units, so that units of unequal lengths leave none idle.  (Units one behind the other on an XCD instead: 2000 tokens in segments of 768, one of three sequences being
+// 1500 long, backward 129 us; so 68.)  Fewer than 16 blocks would leave XCDs without one: these are dealt out as they come.
+constexpr int XCDS = 8;
+inline __host__ __device__ int blocks_an_xcd(int blocks) { return blocks < 2 * XCDS ? 0 : (blocks + XCDS - 1) / XCDS; }
+inline long long scan_workgroups(int blocks, long long units) { return blocks_an_xcd(blocks) ? (long long)XCDS * blocks_an_xcd(blocks) * units : blocks * units; }
+__device__ __forceinline__ bool scan_work(int id, int blocks, int& unit, int& block) {
+    const int most = blocks_an_xcd(blocks);
+    if (!most) {
+        unit = id / blocks;
+        block = id - unit * blocks;
+        return true;
+    }
+    const int xcd = id % XCDS, k = id / XCDS, first = xcd * blocks / XCDS;
+    unit = k / most;
+    block = first + k - unit * most;
+    return block < (xcd + 1) * blocks / XCDS;
 }
 
 // A wave's rows of an operand, tile after tile: the address of its first token's and how far the next tile's are.  (Formed anew in every tile the products
@@ -210,6 +227,42 @@ template <typename T> struct Cursor {
     // beside it that lives through the loop.)
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows() const { return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, NOWHERE_FROM, 0x00027000); }
 };
+
+// The piece of work that a workgroup has: a sequence, or (p.seg) a segment of one.  Packed sequences' counts of segments are not known to the host: sequence n has
+// the units from bos / seg + n on, which never overlap; those that no segment has are idle (`ok`).
+struct Unit {
+    int n, index, len, from, to;      // of its sequence: number of the segment, tokens, first token, one behind the last
+    int64_t bos;
+    bool ok;
+    __device__ __forceinline__ Unit(const ScanArgs& p, int unit) {
+        n = unit;
+        index = 0;
+        if (p.seg && !p.cu) {
+            const int per = (p.T + p.seg - 1) / p.seg;
+            n = unit / per;
+            index = unit - n * per;
+        } else if (p.seg) {
+            int lo = 0, hi = p.N - 1;                     // the last sequence that begins at or before this unit
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (first(p, mid) <= unit) lo = mid;
+                else hi = mid - 1;
+            }
+            n = lo;
+            index = unit - (int)first(p, n);
+        }
+        bos = 0;
+        int64_t eos = p.T;
+        if (p.cu) packed_bounds(p.cu, n, p.T, bos, eos);
+        len = (int)(eos - bos);
+        ok = index >= 0 && (index == 0 || (long long)index * p.seg < len);
+        from = p.seg ? index * p.seg : 0;
+        to = p.seg ? min(len, from + p.seg) : len;
+    }
+    static __device__ __forceinline__ int64_t first(const ScanArgs& p, int n) { return min(max(p.cu[n], (int64_t)0), (int64_t)p.T) / p.seg + n; }
+    __device__ __forceinline__ int segments(const ScanArgs& p) const { return p.seg ? max(1, (len + p.seg - 1) / p.seg) : 1; }
+};
+__device__ __forceinline__ float* ends_of(const ScanArgs& p, long long unit, int block) { return p.ends + (unit * p.blocks + block) * 512; }
 
 // Where a lane stands: as a scanner (channel c, states 4 q .. 4 q + 3) and as a carrier of operands and results (token tok of the piece, V channels from ch)
 template <int LPC, int TOKENS> struct ScanLane {
@@ -275,10 +328,32 @@ inline int lanes_of(int S) { return S <= 8 ? 2 : S <= 16 ? 4 : S <= 32 ? 8 : 16;
 
 // What both passes and the workspace sizes go by
 struct ScanPlan {
-    int lpc, per_group, blocks, slots;
+    int lpc, per_group, blocks, slots, seg;
     bool vec;
-    long long rows, ckpt;
+    long long rows, ckpt, units;
 };
+// Segments fill the device where there are few (sequence, channel block) pairs, at `cost` times the work.  In tokens that a compute unit walks: whole sequences (of packed
+// ones the longest is taken for twice the average) against segments of the length that is best, which have to gain an eighth.
+inline void scan_segments(const hdla_scan_dims* d, ScanPlan& s, float cost) {
+    constexpr long long CUS = 256;
+    const bool packed = d->cu_seqlens != nullptr;
+    const long long average = d->T / (packed ? d->N : 1), longest = packed && d->N > 1 ? std::min<long long>(2 * average, d->T) : d->T;
+    const long long wide = scan_workgroups(s.blocks, 1);
+    auto rounds = [](long long wgs) { return (wgs + CUS - 1) / CUS; };
+    const long long all = wide * d->N;
+    float best = 0.875f * (float)std::max<long long>(longest, rounds(all) * average);
+    s.seg = 0;
+    s.units = d->N;
+    for (long long seg = 2 * SS_SEGMENT; seg < longest; seg += seg < 8 * SS_SEGMENT ? SS_SEGMENT : seg / 4 / SS_SEGMENT * SS_SEGMENT) {
+        const long long busy = packed ? d->T / seg + (d->N + 1) / 2 : d->N * ((d->T + seg - 1) / seg), units = packed ? d->T / seg + d->N : busy;
+        if (units * (s.blocks + 8) > 0x7fffffffLL) continue;
+        // (and what is chained in front of a segment, some two tokens each of those before it, and a launch)
+        const float t = cost * (float)(rounds(busy * wide) * seg) + 2.f * (float)(longest / seg) + 128.f;
+        if (t < best) { best = t; s.seg = (int)seg; s.units = units; }
+    }
+}
+inline size_t ends_bytes(const ScanPlan& s) { return s.seg ? (size_t)s.units * s.blocks * 512 * 4 : 0; }
+constexpr float SEGMENT_COST_FORWARD = 1.6f, SEGMENT_COST_BACKWARD = 1.25f;
 inline bool fits(const void* p, int to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
 inline int scan_plan(const hdla_scan_dims* d, ScanPlan& s) {
@@ -296,9 +371,11 @@ inline int scan_plan(const hdla_scan_dims* d, ScanPlan& s) {
     s.per_group = (size + channels - 1) / channels;
     s.blocks = d->G * s.per_group;
     s.rows = (long long)d->B * d->T;
-    if ((long long)s.blocks * d->N > 0x7fffffffLL || s.rows > 0x7fffffffLL) return HDLA_ERR_SHAPE;
+    if ((long long)(s.blocks + 8) * d->N > 0x7fffffffLL || s.rows > 0x7fffffffLL) return HDLA_ERR_SHAPE;
     s.ckpt = ckpt_slots(d->cu_seqlens != nullptr, d->T, d->N);
     s.slots = 1;
+    s.seg = 0;
+    s.units = d->N;
     return HDLA_OK;
 }
 // Loads of V elements (channels) and of four (states): where everything lies on multiples of them
@@ -324,6 +401,7 @@ inline ScanArgs scan_args(const hdla_scan_dims* d, const ScanPlan& s, const void
     a.A_f32 = d->A_dtype == HDLA_FP32; a.D_f32 = d->D_dtype == HDLA_FP32; a.bias_f32 = d->bias_dtype == HDLA_FP32;
     a.cu = d->cu_seqlens; a.T = d->T; a.N = d->N; a.DD = d->D; a.S = d->S; a.G = d->G; a.softplus = d->softplus != 0;
     a.per_group = s.per_group; a.blocks = s.blocks; a.rows = s.rows; a.slots = s.slots;
+    a.seg = s.seg; a.units = (int)s.units;
     return a;
 }
 

@@ -2,8 +2,9 @@
 //
 // What bounds the scan: the vector ALU.  A state and token cost one multiplication and one exponential (four issue slots) for the decay and six more
 // slots for the two walks, against 8 bytes of x, dt, z, y a channel and token of bf16.
-#include "state_space.cuh"
 #include "hdla_launch.h"
+#include "state_space.cuh"
+#include "state_space_ends.h"
 
 namespace hdla {
 
@@ -18,14 +19,16 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
     __shared__ __attribute__((aligned(16))) Mine mine[W];
     __shared__ Meet meet;
 
-    const int work = xcd_share(blockIdx.x, gridDim.x), n = work / p.blocks, block = work - n * p.blocks;
+    int unit, block;
+    if (!scan_work(blockIdx.x, p.blocks, unit, block)) return;
+    const Unit U(p, unit);
+    if (!U.ok) return;
+    const int n = U.n;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), tid = threadIdx.x;
     const Lane L(p, block);
     Mine& my = mine[w];
-    int64_t bos = 0, eos = p.T;
-    if (p.cu) packed_bounds(p.cu, n, p.T, bos, eos);
-    const int len = (int)(eos - bos);
-    const bool whole = (p.S & 3) == 0;
+    const int64_t bos = U.bos;
+    const int len = U.to;
     const long long batch = p.cu ? 0 : n, row0 = p.cu ? bos : (long long)n * p.T;
     f32x4 A2 = zero4();
     float bias[V], D[V];
@@ -42,14 +45,19 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
     const bool chains = tid < 256, there = chains && (block % p.per_group) * CHN + ec < p.DD / p.G && es < p.S;
     const long long state = ((long long)n * p.DD + L.d0 + ec) * p.S + es;
     float enters = there && p.h0 ? p.h0[state] : 0.f;
+    if (chains)
+        for (int i = 0; i < U.index; ++i) {
+            const float* const left = ends_of(p, unit - U.index + i, block) + tid;
+            enters = __builtin_fmaf(left[256], enters, left[0]);
+        }
 
     Raw<T, V, VEC> rx, rdt, rz;
     StatesOf<T, LPC, TOK, VEC> rB, rC;
-    const long long first = bos + w * TOK;
+    const long long first = bos + U.from + w * TOK;
     Cursor<T> cx(row_of<T>(p.x, batch, first) + L.d0, p.x.row * TILE), cdt(row_of<T>(p.dt, batch, first) + L.d0, p.dt.row * TILE),
         cz(row_of<T>(p.z, batch, first) + L.d0, p.z.row * TILE), cB(row_of<T>(p.B, batch, first) + L.group * p.B_group, p.B.row * TILE),
         cC(row_of<T>(p.C, batch, first) + L.group * p.C_group, p.C.row * TILE),
-        cy(static_cast<const T*>(p.y) + (row0 + w * TOK) * p.DD + L.d0, (long long)p.DD * TILE);
+        cy(static_cast<const T*>(p.y) + (row0 + U.from + w * TOK) * p.DD + L.d0, (long long)p.DD * TILE);
     const uint32_t ox = L.offset(p.x.row, sizeof(T)), odt = L.offset(p.dt.row, sizeof(T)), oz = L.offset(p.z.row, sizeof(T)), oy = L.offset(p.DD, sizeof(T));
     auto request = [&](int t0) __attribute__((always_inline)) {
         const int tokens = min(max(len - t0, 0), TOK);
@@ -62,8 +70,8 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
         rC.load(cC, (uint32_t)p.C.row, tokens, p.S);
         cx.next(); cdt.next(); cz.next(); cB.next(); cC.next();
     };
-    request(w * TOK);
-    for (int tile = 0; tile < len; tile += TILE) {
+    request(U.from + w * TOK);
+    for (int tile = U.from; tile < len; tile += TILE) {
         const int t0 = tile + w * TOK, tokens = min(max(len - t0, 0), TOK);
         float x[V], z[V];
 #pragma unroll
@@ -161,7 +169,7 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
         cy.next();
         wave_lds_fence();                                 // the next tile's operands go where y is
     }
-    if (there && p.ht) p.ht[state] = enters;
+    if (there && p.ht && U.to == U.len) p.ht[state] = enters;
 }
 
 // One token of each sequence: lpc lanes a channel, four states each; a thread takes NB sequences one behind the other, whose states are on their way together and whose
@@ -226,13 +234,17 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs p, int lpc_log2
 }
 
 template <typename T, int LPC, int L, int W> static void launch_tokens(const ScanArgs& a, bool vec, hipStream_t s) {
-    const dim3 grid((unsigned)((long long)a.blocks * a.N)), block(64 * W);
+    const dim3 grid((unsigned)scan_workgroups(a.blocks, a.units)), block(64 * W);
     if (vec) hipLaunchKernelGGL((scan_tokens_kernel<T, LPC, L, W, true>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((scan_tokens_kernel<T, LPC, L, W, false>), grid, block, 0, s, a);
 }
 template <typename T> static hipError_t launch_scan(const ScanArgs& a, const ScanPlan& s, hipStream_t st) {
     const int average = a.T / (a.cu ? a.N : 1);
     const bool few = average <= 64;
+    if (s.seg) {
+        const hipError_t e = launch_scan_ends<T>(a, s, false, st);
+        if (e != hipSuccess) return e;
+    }
     switch (s.lpc) {
 #define HDLA_SCAN_CASE(LPCV)                                                          \
     case LPCV:                                                                        \
@@ -254,16 +266,24 @@ template <typename T> static hipError_t launch_scan(const ScanArgs& a, const Sca
 using namespace hdla;
 
 extern "C" int hdla_state_space_version(void) { return HDLA_STATE_SPACE_VERSION; }
+extern "C" size_t hdla_scan_fwd_workspace_bytes(const hdla_scan_dims* dims) {
+    ScanPlan s;
+    if (scan_plan(dims, s)) return 0;
+    scan_segments(dims, s, SEGMENT_COST_FORWARD);
+    return ends_bytes(s);
+}
 extern "C" int hdla_scan_fwd(const hdla_scan_dims* dims, const void* x, const void* dt, const void* A, const void* B, const void* C, const void* D, const void* z,
-                             const void* dt_bias, const float* h0, void* y, float* ht, void* states, size_t states_bytes, void* stream) {
+                             const void* dt_bias, const float* h0, void* y, float* ht, void* states, size_t states_bytes, void* workspace, size_t workspace_bytes, void* stream) {
     ScanPlan s;
     const int rc = scan_plan(dims, s);
     if (rc) return rc;
     if (s.rows > 0 && (!x || !dt || !A || !B || !C || !y)) return HDLA_ERR_NULL;
     if (!fits(y, 16) || !fits(h0, 16) || !fits(ht, 16)) return HDLA_ERR_ALIGN;
     if (states && (!fits(states, 16) || states_bytes < (size_t)s.ckpt * s.blocks * 1024)) return HDLA_ERR_WORKSPACE;
+    scan_segments(dims, s, SEGMENT_COST_FORWARD);
+    if (s.seg && (!workspace || !fits(workspace, 16) || workspace_bytes < ends_bytes(s))) return HDLA_ERR_WORKSPACE;
     ScanArgs a = scan_args(dims, s, x, dt, A, B, C, D, z, dt_bias);
-    a.h0 = h0; a.ht = ht; a.y = y; a.ckpt = static_cast<float*>(states);
+    a.h0 = h0; a.ht = ht; a.y = y; a.ckpt = static_cast<float*>(states); a.ends = static_cast<float*>(workspace);
     s.vec = scan_vec(dims, s, a);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (a.cu) {

@@ -9,6 +9,7 @@
 #include "column_sums.cuh"
 #include "hdla_launch.h"
 #include "state_space.cuh"
+#include "state_space_ends.h"
 
 namespace hdla {
 
@@ -33,7 +34,8 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
     __shared__ __attribute__((aligned(16))) Mine mine[W];
     __shared__ Meet meet;
 
-    const int work = xcd_share(blockIdx.x, gridDim.x), slot = work / p.blocks, block = work - slot * p.blocks;
+    int slot, block;
+    if (!scan_work(blockIdx.x, p.blocks, slot, block)) return;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), tid = threadIdx.x;
     const Lane L(p, block);
     Mine& my = mine[w];
@@ -52,15 +54,21 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
     const int e = tid & 255, ec = (e >> 2) / LPC, es = 4 * ((e >> 2) % LPC) + (e & 3);
     const bool forwards = tid < 256, backwards = tid >= 256 && tid < 512, there = (block % p.per_group) * CHN + ec < p.DD / p.G && es < p.S;
 
-    for (int n = slot; n < p.N; n += p.slots) {
-        int64_t bos = 0, eos = p.T;
-        if (p.cu) packed_bounds(p.cu, n, p.T, bos, eos);
-        const int len = (int)(eos - bos);
+    for (int unit = slot; unit < p.units; unit += p.slots) {
+        const Unit U(p, unit);
+        if (!U.ok) continue;                              // (the same on all threads)
+        const int n = U.n, len = U.to;
+        const int64_t bos = U.bos;
         const long long batch = p.cu ? 0 : n, row0 = p.cu ? bos : (long long)n * p.T;
         const long long state = ((long long)n * p.DD + L.d0 + ec) * p.S + es;
         float enters = backwards && there && p.dht ? p.dht[state] : 0.f;
+        if (backwards)
+            for (int i = U.segments(p) - 1; i > U.index; --i) {
+                const float* const left = ends_of(p, unit - U.index + i, block) + e;
+                enters = __builtin_fmaf(left[256], enters, left[0]);
+            }
 
-        const int tiles = (len + TILE - 1) / TILE;
+        const int tiles = (len + TILE - 1) / TILE, until = U.from / TILE;
         const long long first = bos + (long long)(tiles - 1) * TILE + w * TOK, frow = row0 + (long long)(tiles - 1) * TILE + w * TOK;
         Cursor<T> cx(row_of<T>(p.x, batch, first) + L.d0, -p.x.row * TILE), cdt(row_of<T>(p.dt, batch, first) + L.d0, -p.dt.row * TILE),
             cz(row_of<T>(p.z, batch, first) + L.d0, -p.z.row * TILE), cB(row_of<T>(p.B, batch, first) + L.group * p.B_group, -p.B.row * TILE),
@@ -71,7 +79,7 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
         Raw<T, V, VEC> rx, rdt, rz, rdy;
         StatesOf<T, LPC, TOK, VEC> rB, rC;
         auto request = [&](int t0) __attribute__((always_inline)) {
-            const int tokens = t0 < 0 ? 0 : min(max(len - t0, 0), TOK);
+            const int tokens = t0 < U.from ? 0 : min(max(len - t0, 0), TOK);
             const bool live = L.tok < tokens && L.carried > 0;
             rx.load(cx.rows(), live ? ox : NOWHERE, L.carried);
             rdt.load(cdt.rows(), live ? odt : NOWHERE, L.carried);
@@ -83,7 +91,7 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
             cx.next(); cdt.next(); cz.next(); cdy.next(); cB.next(); cC.next();
         };
         request((tiles - 1) * TILE + w * TOK);
-        for (int tile = tiles - 1; tile >= 0; --tile) {
+        for (int tile = tiles - 1; tile >= until; --tile) {
             const int t0 = tile * TILE + w * TOK, tokens = min(max(len - t0, 0), TOK);
             const float left = forwards ? p.ckpt[((ckpt_slot(p, n, bos) + tile * (TILE / SS_CKPT)) * p.blocks + block) * 256 + e] : 0.f;
             float x[V], z[V], dy[V], v[V], ev[V], gz[V], delta[V], ee[V];
@@ -268,7 +276,7 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
             }
             wave_lds_fence();
         }
-        if (backwards && there && p.dh0) p.dh0[state] = enters;
+        if (backwards && there && p.dh0 && U.index == 0) p.dh0[state] = enters;
     }
     // what the waves have of dA, dD and d bias
     __syncthreads();
@@ -296,17 +304,18 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
     }
 }
 
-// Workgroups walk sequences in turns so that their partial sums of dA, dD and d bias stay few: as many as fill the device a few times
-static int grad_slots(const hdla_scan_dims* d, const ScanPlan& s) {
+// Workgroups walk sequences, or segments, in turns so that their partial sums of dA, dD and d bias stay few: as many as fill the device a few times
+static int grad_slots(const ScanPlan& s) {
     const long long most = std::max(1LL, 2048LL / s.blocks);
-    return (int)std::min<long long>(d->N, most);
+    return (int)std::min<long long>(s.units, most);
 }
-// partial sums of dB and dC, [blocks of a group][2][rows][G][S], and behind them those of dA, dD and d bias, [slots][D S + 2 D]
+// partial sums of dB and dC, [blocks of a group][2][rows][G][S], and behind them those of dA, dD and d bias, [slots][D S + 2 D], and segments' ends
 static size_t bc_bytes(const hdla_scan_dims* d, const ScanPlan& s) { return ((size_t)s.per_group * 2 * s.rows * d->G * d->S * 4 + 15) / 16 * 16; }
-static size_t grad_bytes(const hdla_scan_dims* d, const ScanPlan& s, int slots) { return bc_bytes(d, s) + (size_t)slots * d->D * (d->S + 2) * 4; }
+static size_t own_bytes(const hdla_scan_dims* d, int slots) { return ((size_t)slots * d->D * (d->S + 2) * 4 + 15) / 16 * 16; }
+static size_t grad_bytes(const hdla_scan_dims* d, const ScanPlan& s, int slots) { return bc_bytes(d, s) + own_bytes(d, slots) + ends_bytes(s); }
 template <typename T, int LPC> static void launch_grad(const ScanArgs& a, bool vec, hipStream_t s) {
     constexpr int TOK = SS_TOK, W = 8;
-    const dim3 grid((unsigned)((long long)a.blocks * a.slots)), block(64 * W);
+    const dim3 grid((unsigned)scan_workgroups(a.blocks, a.slots)), block(64 * W);
     if (vec) hipLaunchKernelGGL((scan_grad_kernel<T, LPC, TOK, W, true>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((scan_grad_kernel<T, LPC, TOK, W, false>), grid, block, 0, s, a);
 }
@@ -327,7 +336,9 @@ using namespace hdla;
 
 extern "C" size_t hdla_scan_workspace_bytes(const hdla_scan_dims* dims) {
     ScanPlan s;
-    return scan_plan(dims, s) ? 0 : grad_bytes(dims, s, grad_slots(dims, s));
+    if (scan_plan(dims, s)) return 0;
+    scan_segments(dims, s, SEGMENT_COST_BACKWARD);
+    return grad_bytes(dims, s, grad_slots(s));
 }
 extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const void* dt, const void* A, const void* B, const void* C, const void* D, const void* z,
                              const void* dt_bias, const void* dy, const float* dht, const void* states, size_t states_bytes, void* dx, void* ddt, void* dA, void* dB,
@@ -339,7 +350,8 @@ extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const vo
     if (s.rows > 0 && (!x || !dt || !B || !C || !dy || !dx || !ddt || !dB || !dC || !states || (z && !dz))) return HDLA_ERR_NULL;
     for (const void* q : {dy, (const void*)dht, states, (const void*)dx, (const void*)ddt, (const void*)dB, (const void*)dC, (const void*)dz, (const void*)dh0})
         if (!fits(q, 16)) return HDLA_ERR_ALIGN;
-    s.slots = grad_slots(dims, s);
+    scan_segments(dims, s, SEGMENT_COST_BACKWARD);
+    s.slots = grad_slots(s);
     if (!workspace || !fits(workspace, 16) || workspace_bytes < grad_bytes(dims, s, s.slots)) return HDLA_ERR_WORKSPACE;
     if (s.rows > 0 && states_bytes < (size_t)s.ckpt * s.blocks * 1024) return HDLA_ERR_WORKSPACE;
     ScanArgs a = scan_args(dims, s, x, dt, A, B, C, D, z, dt_bias);
@@ -348,6 +360,7 @@ extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const vo
     char* const base = static_cast<char*>(workspace);
     a.part_bc = reinterpret_cast<float*>(base);
     a.part_own = reinterpret_cast<float*>(base + bc_bytes(dims, s));
+    a.ends = reinterpret_cast<float*>(base + bc_bytes(dims, s) + own_bytes(dims, s.slots));
     s.vec = scan_vec(dims, s, a);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const int es = dims->dtype == HDLA_BF16 ? 2 : 4;
@@ -355,6 +368,10 @@ extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const vo
         PackedOut out{};
         for (void* o : {dx, ddt, dz}) out.add(o, (long long)dims->D * es);
         const hipError_t e = launch_clear_uncovered(a.cu, a.N, a.T, out, st);
+        if (e != hipSuccess) return (int)e;
+    }
+    if (s.seg) {
+        const hipError_t e = dims->dtype == HDLA_BF16 ? launch_scan_ends<bf16>(a, s, true, st) : launch_scan_ends<float>(a, s, true, st);
         if (e != hipSuccess) return (int)e;
     }
     hipError_t e = dims->dtype == HDLA_BF16 ? launch_scan_grad<bf16>(a, s, st) : launch_scan_grad<float>(a, s, st);

@@ -13,7 +13,7 @@ import torch
 
 HDLA_BF16, HDLA_FP32 = 0, 1
 HDLA_VERSION = 211          # the header this binding was written against (struct layouts, entry points)
-STATE_SPACE_VERSION = 1      # the same of include/hdla_state_space.h
+STATE_SPACE_VERSION = 2      # the same of include/hdla_state_space.h
 ROUTE_AUTO, ROUTE_CLASSIC, ROUTE_FUSED, ROUTE_PLAIN = 0, 1, 2, 4
 _ROUTES = {"": ROUTE_AUTO, "auto": ROUTE_AUTO, "classic": ROUTE_CLASSIC, "plain": ROUTE_PLAIN, "fused": ROUTE_FUSED}
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -195,7 +195,7 @@ def load():
     for name, result, arguments in (
             ("short_conv_fwd", ctypes.c_int, [CF] + [P] * 7), ("short_conv_workspace_bytes", Z, [CF]), ("short_conv_bwd", ctypes.c_int, [CF] + [P] * 11 + [Z, P]),
             ("short_conv_step", ctypes.c_int, [CF] + [P] * 7),
-            ("scan_states_bytes", Z, [SF]), ("scan_fwd", ctypes.c_int, [SF] + [P] * 12 + [Z, P]), ("scan_workspace_bytes", Z, [SF]),
+            ("scan_states_bytes", Z, [SF]), ("scan_fwd", ctypes.c_int, [SF] + [P] * 12 + [Z, P, Z, P]), ("scan_fwd_workspace_bytes", Z, [SF]), ("scan_workspace_bytes", Z, [SF]),
             ("scan_bwd", ctypes.c_int, [SF] + [P] * 11 + [Z] + [P] * 10 + [Z, P]), ("scan_step", ctypes.c_int, [SF] + [P] * 12),
             ("block_norm_fwd", ctypes.c_int, [BF] + [P] * 9), ("block_norm_workspace_bytes", Z, [BF]),
             ("block_norm_bwd", ctypes.c_int, [BF] + [P] * 15 + [Z, P])):

@@ -297,8 +297,9 @@ class StateSpaceScanFunction(torch.autograd.Function):
             left = None
             if any(ctx.needs_input_grad):
                 left = torch.empty(lib.hdla_scan_states_bytes(ctypes.byref(dims)), dtype=torch.uint8, device=x.device)
+            ws = torch.empty(lib.hdla_scan_fwd_workspace_bytes(ctypes.byref(dims)), dtype=torch.uint8, device=x.device)
             _lib.check(lib.hdla_scan_fwd(ctypes.byref(dims), _lib.ptr(x), _lib.ptr(dt), _lib.ptr(A), _lib.ptr(B), _lib.ptr(C), _lib.ptr(D), _lib.ptr(z), _lib.ptr(bias),
-                                         _lib.ptr(h0), _lib.ptr(y), _lib.ptr(ht), _lib.ptr(left), 0 if left is None else left.numel(),
+                                         _lib.ptr(h0), _lib.ptr(y), _lib.ptr(ht), _lib.ptr(left), 0 if left is None else left.numel(), _lib.ptr(ws), ws.numel(),
                                          _lib.current_stream(x.device)), "hdla_scan_fwd")
         ctx.save_for_backward(x, dt, A, B, C, D, z, bias, h0, cu, left)
         ctx.cfg = (softplus, n)

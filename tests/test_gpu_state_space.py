@@ -57,6 +57,44 @@ def test_scan_and_gradients(nb, T, d, S, G, dtype):
     compare(low, ref, dy, dh, True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("nb,T,d,S,G,state", [(1, 1500, 16, 16, 1, True), (2, 1030, 9, 8, 1, False), (1, 1281, 8, 33, 2, True), (1, 900, 12, 20, 1, True)])
+def test_long_sequences_of_few_channels(nb, T, d, S, G, state, dtype):
+    """Cut into segments that run side by side."""
+    low, ref, dy, dh = make(T + d, nb, T, d, S, G, dtype, state=state)
+    compare(low, ref, dy, dh, True)
+
+
+@pytest.mark.parametrize("inner", [(3, 700, 701), (256, 512, 1024), (1400, 1499, 1500), (0, 0, 1)])
+def test_long_packed_sequences_of_few_channels(inner):
+    T = 1501
+    cu = cuts(T, inner)
+    low, ref, dy, dh = make(sum(inner), 1, T, 16, 16, 1, torch.float32, N=len(inner) + 1)
+    compare(low, ref, dy, dh, True, cu)
+    v = put(low)
+    v2 = put(low)
+    for a, b in zip(call(v, True, True, cu), call(v2, True, True, cu.to(DEV))):
+        assert torch.equal(a, b)
+
+
+def test_long_tables_that_leave_tokens_out_or_decrease():
+    low, ref, dy, dh = make(24, 1, 1500, 16, 16, 1, torch.float32, N=3)
+    v = put(low)
+    cu = torch.tensor([300, 301, 1100, 1400])
+    y, ht = call(v, True, True, cu.to(DEV))
+    g = torch.autograd.grad([y, ht], [v["x"], v["B"], v["C"]], [dy.to(DEV), dh.to(DEV)])
+    yr, hr = O.scan(*[ref[k] for k in NAMES[:8]], True, ref["h0"], cu)
+    m, count = O.scan_magnitudes(*[ref[k] for k in NAMES[:8]], True, ref["h0"], cu, dy.double(), dh.double())
+    close("y", y, yr, m["y"], count)
+    close("ht", ht, hr, m["ht"], count)
+    for k, a, b in zip(("x", "B", "C"), g, torch.autograd.grad([yr, hr], [ref["x"], ref["B"], ref["C"]], [dy.double(), dh.double()])):
+        close("d" + k, a, b, m[k], count)
+    y, ht = call(v, True, True, torch.tensor([-7, 1300, 200, 5000], device=DEV))
+    g = torch.autograd.grad(y, [v[k] for k in NAMES], dy.to(DEV))
+    torch.cuda.synchronize()
+    assert torch.isfinite(y).all() and all(torch.isfinite(t).all() for t in g)
+
+
 @pytest.mark.parametrize("gate,skip,bias,state,softplus", [(False, False, False, False, False), (True, False, False, True, True), (False, True, True, False, True),
                                                            (True, True, False, False, False)])
 def test_what_may_be_left_out(gate, skip, bias, state, softplus):

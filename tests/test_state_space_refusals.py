@@ -12,7 +12,7 @@ from hdla_hip import _lib, block_norm, short_conv, short_conv_step, state_space_
 
 HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "hdla_state_space.h")
 # the declarations of each number, without comments and white space: a change of them takes the next number and a line here
-DECLARED = {1: "dcb9c70b5ad9866a"}
+DECLARED = {1: "dcb9c70b5ad9866a", 2: "c4ab95f61548d8a0"}
 
 
 def test_the_number_is_of_these_declarations():
@@ -111,7 +111,7 @@ def test_c_entry_points_answer_wrong_dimensions_with_codes():
     for wrong, rc in ((dict(S=65), -2), (dict(S=0), -2), (dict(G=3), -2), (dict(A_dtype=9), -4), (dict(N=3), -7), (dict(B=0), -2)):
         d = _lib.HdlaScanDims(**dict(scan, **wrong))
         assert lib.hdla_scan_workspace_bytes(by(d)) == 0 and lib.hdla_scan_states_bytes(by(d)) == 0
-        assert lib.hdla_scan_fwd(by(d), *[None] * 12, 0, None) == rc
+        assert lib.hdla_scan_fwd(by(d), *[None] * 12, 0, None, 0, None) == rc
         assert lib.hdla_scan_bwd(by(d), *[None] * 11, 0, *[None] * 10, 0, None) == rc
         assert lib.hdla_scan_step(by(d), *[None] * 12) == rc
     assert lib.hdla_scan_step(by(_lib.HdlaScanDims(**scan)), *[None] * 12) == -2              # one token
@@ -129,7 +129,7 @@ def test_c_entry_points_answer_small_and_misaligned_buffers_with_codes():
     p = lambda a: ctypes.c_void_p(a)
     scan = _lib.HdlaScanDims(B=1, T=100, D=8, S=16, G=1, N=1, dtype=0, A_dtype=1, D_dtype=1, bias_dtype=1, softplus=1)
     ok = p(4096)
-    args = lambda y, states, n: [ok] * 5 + [None] * 4 + [y, None, states, n, None]
+    args = lambda y, states, n: [ok] * 5 + [None] * 4 + [y, None, states, n, None, 0, None]
     assert lib.hdla_scan_fwd(by(scan), *args(p(4100), None, 0)) == -6
     assert lib.hdla_scan_fwd(by(scan), *args(ok, ok, 16)) == -5
     assert lib.hdla_scan_bwd(by(scan), *[ok] * 11, 1 << 40, *[ok] * 10, 16, None) == -5
