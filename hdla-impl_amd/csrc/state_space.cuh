@@ -21,7 +21,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // floats from one channel to the next of a piece of L tokens in LDS: 16 bytes aligned, neighbours on other banks
 constexpr int ss_pitch(int L) { return L + 4; }
-constexpr int SS_TOK = 8;             // tokens of a wave at a time; the forward pass takes twice as many of long sequences (not of 32 channels a wave: registers)
+constexpr int SS_TOK = 8;             // tokens of a wave at a time
 constexpr int SS_CKPT = 64;           // tokens between the states that a forward pass leaves for the backward pass
 
 // element (b, t, .) of an operand: base + b batch + t row.  A wave's tokens are reached by 32-bit offsets from its first one's row.
@@ -380,7 +380,7 @@ inline int scan_plan(const hdla_scan_dims* d, ScanPlan& s) {
 }
 // Loads of V elements (channels) and of four (states): where everything lies on multiples of them
 inline bool scan_vec(const hdla_scan_dims* d, const ScanPlan& s, const ScanArgs& a) {
-    const int es = d->dtype == HDLA_BF16 ? 2 : 4, v = std::min(4, 2 * SS_TOK / s.lpc), size = d->D / d->G;
+    const int es = d->dtype == HDLA_BF16 ? 2 : 4, v = std::max(1, SS_TOK / s.lpc), size = d->D / d->G;
     if (size % v || d->S % 4) return false;
     const int bytes = std::min(v * es, 16);
     for (const Operand* o : {&a.x, &a.dt, &a.z})

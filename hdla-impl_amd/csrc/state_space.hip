@@ -18,6 +18,7 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
     struct Meet { f32x4 P[W][64], E[W][64]; };
     __shared__ __attribute__((aligned(16))) Mine mine[W];
     __shared__ Meet meet;
+    __shared__ float bias[CHN], skip[CHN];                // (in registers they are what does not fit)
 
     int unit, block;
     if (!scan_work(blockIdx.x, p.blocks, unit, block)) return;
@@ -31,15 +32,15 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
     const int len = U.to;
     const long long batch = p.cu ? 0 : n, row0 = p.cu ? bos : (long long)n * p.T;
     f32x4 A2 = zero4();
-    float bias[V], D[V];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (j < L.left) A2[j] = ld_param(p.A, p.A_f32, (long long)L.d * p.S + 4 * L.q + j) * LOG2E;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bias[i] = p.bias && i < L.carried ? ld_param(p.bias, p.bias_f32, L.dv + i) : 0.f;
-        D[i] = p.D && i < L.carried ? ld_param(p.D, p.D_f32, L.dv + i) : 0.f;
+    if (tid < CHN) {
+        const bool in = (block % p.per_group) * CHN + tid < p.DD / p.G;
+        bias[tid] = p.bias && in ? ld_param(p.bias, p.bias_f32, L.d0 + tid) : 0.f;
+        skip[tid] = p.D && in ? ld_param(p.D, p.D_f32, L.d0 + tid) : 0.f;
     }
+    __syncthreads();
     // The state that enters the tile, one of the 256 states of the block a thread of the first four waves: number tid of meet.E's rows
     const int ec = (tid >> 2) / LPC, es = 4 * ((tid >> 2) % LPC) + (tid & 3);
     const bool chains = tid < 256, there = chains && (block % p.per_group) * CHN + ec < p.DD / p.G && es < p.S;
@@ -79,7 +80,7 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
             x[i] = rx[i];
             z[i] = rz[i];
             float e;
-            const float v = rdt[i] + bias[i], delta = L.tok < tokens ? (p.softplus ? softplus<T>(v, e) : v) : 0.f;
+            const float v = rdt[i] + bias[L.ch + i], delta = L.tok < tokens ? (p.softplus ? softplus<T>(v, e) : v) : 0.f;
             if (L.tok < TOK) {
                 my.d[(L.ch + i) * PITCH + L.tok] = delta;
                 my.x[(L.ch + i) * PITCH + L.tok] = delta * x[i];
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
         if (p.z.p) sigmoid_each<T, V>(z, g);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            o[i] = __builtin_fmaf(D[i], x[i], my.d[(L.ch + i) * PITCH + min(L.tok, TOK - 1)]);
+            o[i] = __builtin_fmaf(skip[L.ch + i], x[i], my.d[(L.ch + i) * PITCH + min(L.tok, TOK - 1)]);
             if (p.z.p) o[i] *= z[i] * g[i];
         }
         if (L.tok < tokens && L.carried > 0)
@@ -233,23 +234,29 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs p, int lpc_log2
     }
 }
 
-template <typename T, int LPC, int L, int W> static void launch_tokens(const ScanArgs& a, bool vec, hipStream_t s) {
-    const dim3 grid((unsigned)scan_workgroups(a.blocks, a.units)), block(64 * W);
-    if (vec) hipLaunchKernelGGL((scan_tokens_kernel<T, LPC, L, W, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((scan_tokens_kernel<T, LPC, L, W, false>), grid, block, 0, s, a);
+template <typename T, int LPC, int W, bool VEC> static void launch_tokens(const ScanArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((scan_tokens_kernel<T, LPC, SS_TOK, W, VEC>), dim3((unsigned)scan_workgroups(a.blocks, a.units)), dim3(64 * W), 0, s, a);
+}
+// Waves of a workgroup.  Where the registers of four waves a SIMD suffice: eight, two workgroups a compute unit, if there are as many; else sixteen.  Where they don't: twelve.
+// Short sequences: four.  us, eight / twelve / sixteen (and 16 tokens a wave, eight waves): 8192 x 4096 channels, 256 workgroups, 245 / 214 / 195 (215); 4 x 2048 x 2048, 512 of them,
+// 72 / 84 / 77 (94).
+template <typename T, int LPC, bool VEC> static void launch_lpc(const ScanArgs& a, hipStream_t s) {
+    constexpr bool lean = LPC == 8 || (VEC && sizeof(T) == 2 && LPC >= 4);
+    if (a.T / (a.cu ? a.N : 1) <= 64) launch_tokens<T, LPC, 4, VEC>(a, s);
+    else if constexpr (!lean) launch_tokens<T, LPC, 12, VEC>(a, s);
+    else if (scan_workgroups(a.blocks, a.units) >= 512) launch_tokens<T, LPC, 8, VEC>(a, s);
+    else launch_tokens<T, LPC, 16, VEC>(a, s);
 }
 template <typename T> static hipError_t launch_scan(const ScanArgs& a, const ScanPlan& s, hipStream_t st) {
-    const int average = a.T / (a.cu ? a.N : 1);
-    const bool few = average <= 64;
     if (s.seg) {
         const hipError_t e = launch_scan_ends<T>(a, s, false, st);
         if (e != hipSuccess) return e;
     }
     switch (s.lpc) {
-#define HDLA_SCAN_CASE(LPCV)                                                          \
-    case LPCV:                                                                        \
-        if (few) launch_tokens<T, LPCV, SS_TOK, 4>(a, s.vec, st);                             \
-        else launch_tokens<T, LPCV, LPCV == 2 ? SS_TOK : 2 * SS_TOK, 8>(a, s.vec, st);                                 \
+#define HDLA_SCAN_CASE(LPCV)                                  \
+    case LPCV:                                                \
+        if (s.vec) launch_lpc<T, LPCV, true>(a, st);          \
+        else launch_lpc<T, LPCV, false>(a, st);               \
         break;
         HDLA_SCAN_CASE(2)
         HDLA_SCAN_CASE(4)
