@@ -113,7 +113,7 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
             rC.put(my.C);
             request(t0 - TILE);
             wave_lds_fence();
-            f32x4 a[TOK], E = zero4(), G = zero4();
+            f32x4 a[TOK], add[TOK], E = zero4(), G = zero4();         // decays; what each token adds
             const float *const mine_d = &my.d[L.c * PITCH], *const mine_x = &my.x[L.c * PITCH], *const mine_e = &my.e[L.c * PITCH];
             float sum = 0.f;
             // (in all the walks: the next token's operands are on their way while this one's are worked on)
@@ -129,7 +129,8 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         a[k][j] = __builtin_amdgcn_exp2f(dl * A2[j]);
-                        E[j] = __builtin_fmaf(a[k][j], E[j], u * b[j]);
+                        add[k][j] = u * b[j];
+                        E[j] = __builtin_fmaf(a[k][j], E[j], add[k][j]);
                     }
                     apart();
                     if (k + 1 < TOK) { b = b1; dl = dl1; u = u1; }
@@ -182,23 +183,21 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
             G = meet.G[w][l];
             f32x4 h[TOK];
             {
-                f32x4 b = my.B[L.q], cc = my.C[L.q];
-                float u = mine_x[0];
+                f32x4 cc = my.C[L.q];
 #pragma unroll
                 for (int k = 0; k < TOK; ++k) {
-                    f32x4 b1, c1;
-                    float u1;
-                    if (k + 1 < TOK) { b1 = my.B[(k + 1) * LPC + L.q]; c1 = my.C[(k + 1) * LPC + L.q]; u1 = mine_x[k + 1]; }
+                    f32x4 c1;
+                    if (k + 1 < TOK) c1 = my.C[(k + 1) * LPC + L.q];
                     float y[1] = {0.f};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        h[k][j] = __builtin_fmaf(a[k][j], k ? h[k - 1][j] : first[j], u * b[j]);
+                        h[k][j] = __builtin_fmaf(a[k][j], k ? h[k - 1][j] : first[j], add[k][j]);
                         y[0] = __builtin_fmaf(h[k][j], cc[j], y[0]);
                     }
                     sum_channel<LPC>(y);
                     my.y[L.c * PITCH + k] = y[0];        // (the same from all lanes of the channel)
                     apart();
-                    if (k + 1 < TOK) { b = b1; cc = c1; u = u1; }
+                    if (k + 1 < TOK) cc = c1;
                 }
             }
             wave_lds_fence();                             // B and C are read again, not kept
