@@ -22,7 +22,9 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 // floats from one channel to the next of a piece of L tokens in LDS: 16 bytes aligned, neighbours on other banks
 constexpr int ss_pitch(int L) { return L + 4; }
 constexpr int SS_TOK = 8;             // tokens of a wave at a time
-constexpr int SS_CKPT = 64;           // tokens between the states that a forward pass leaves for the backward pass
+// Tokens between the states that a forward pass leaves for the backward pass: a tile of that pass, of four waves where there are workgroups for two on every compute unit,
+// whose barriers then fall into each other's work, else of eight.  us a training step, eight / four: 4 x 2048 x 2048 (512 workgroups of four waves) 432 / 416, 2503 x 520 in fp32 (264) 152 / 181.
+constexpr int SS_TILE_FEW = 64, SS_TILE_MANY = 32;
 
 // element (b, t, .) of an operand: base + b batch + t row.  A wave's tokens are reached by 32-bit offsets from its first one's row.
 struct Operand {
@@ -45,6 +47,7 @@ struct ScanArgs {
     const int64_t* cu;
     int T, N, DD, S, G, softplus;
     int per_group, blocks;            // channel blocks of a group, of all of them
+    int every;                        // SS_TILE_FEW or SS_TILE_MANY
     // backward
     const void* dy;                   // [rows, D]
     const float* dht;
@@ -317,10 +320,10 @@ template <int LPC, int N> __device__ __forceinline__ void sum_channel(float (&x)
 
 // first slot of a sequence in the states that a forward pass leaves: packed sequences' counts are not known to the host, and these never overlap
 __device__ __forceinline__ long long ckpt_slot(const ScanArgs& p, int n, int64_t bos) {
-    return p.cu ? bos / SS_CKPT + n : (long long)n * ((p.T + SS_CKPT - 1) / SS_CKPT);
+    return p.cu ? bos / p.every + n : (long long)n * ((p.T + p.every - 1) / p.every);
 }
-inline long long ckpt_slots(bool packed, long long T, long long N) {
-    return packed ? T / SS_CKPT + N + 1 : N * ((T + SS_CKPT - 1) / SS_CKPT);
+inline long long ckpt_slots(bool packed, long long T, long long N, int every) {
+    return packed ? T / every + N + 1 : N * ((T + every - 1) / every);
 }
 
 // ---- host side: what both passes and the workspace sizes go by ---------------------------------------------------------
@@ -328,7 +331,7 @@ inline int lanes_of(int S) { return S <= 8 ? 2 : S <= 16 ? 4 : S <= 32 ? 8 : 16;
 
 // What both passes and the workspace sizes go by
 struct ScanPlan {
-    int lpc, per_group, blocks, slots, seg;
+    int lpc, per_group, blocks, slots, seg, every;
     bool vec;
     long long rows, ckpt, units;
 };
@@ -372,7 +375,8 @@ inline int scan_plan(const hdla_scan_dims* d, ScanPlan& s) {
     s.blocks = d->G * s.per_group;
     s.rows = (long long)d->B * d->T;
     if ((long long)(s.blocks + 8) * d->N > 0x7fffffffLL || s.rows > 0x7fffffffLL) return HDLA_ERR_SHAPE;
-    s.ckpt = ckpt_slots(d->cu_seqlens != nullptr, d->T, d->N);
+    s.every = scan_workgroups(s.blocks, d->N) >= 512 ? SS_TILE_MANY : SS_TILE_FEW;
+    s.ckpt = ckpt_slots(d->cu_seqlens != nullptr, d->T, d->N, s.every);
     s.slots = 1;
     s.seg = 0;
     s.units = d->N;
@@ -400,7 +404,7 @@ inline ScanArgs scan_args(const hdla_scan_dims* d, const ScanPlan& s, const void
     a.B_group = d->B_group; a.C_group = d->C_group;
     a.A_f32 = d->A_dtype == HDLA_FP32; a.D_f32 = d->D_dtype == HDLA_FP32; a.bias_f32 = d->bias_dtype == HDLA_FP32;
     a.cu = d->cu_seqlens; a.T = d->T; a.N = d->N; a.DD = d->D; a.S = d->S; a.G = d->G; a.softplus = d->softplus != 0;
-    a.per_group = s.per_group; a.blocks = s.blocks; a.rows = s.rows; a.slots = s.slots;
+    a.per_group = s.per_group; a.blocks = s.blocks; a.every = s.every; a.rows = s.rows; a.slots = s.slots;
     a.seg = s.seg; a.units = (int)s.units;
     return a;
 }

@@ -135,8 +135,8 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
         }
         __syncthreads();
         f32x4 h = meet.E[w][l];
-        if (p.ckpt && t0 % SS_CKPT == 0 && tokens > 0)
-            *reinterpret_cast<f32x4*>(p.ckpt + (((ckpt_slot(p, n, bos) + t0 / SS_CKPT) * p.blocks + block) * 64 + l) * 4) = h;
+        if (p.ckpt && (t0 & (p.every - 1)) == 0 && tokens > 0)
+            *reinterpret_cast<f32x4*>(p.ckpt + (((ckpt_slot(p, n, bos) + t0 / p.every) * p.blocks + block) * 64 + l) * 4) = h;
         float y[TOK];
         f32x4 cc = my.C[L.q];
 #pragma unroll

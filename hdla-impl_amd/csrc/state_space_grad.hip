@@ -2,8 +2,8 @@
 //     G_t = C_t e_t + exp(delta_{t+1} A) G_{t+1};   u_t = exp(delta_t A) h_{t-1};
 //     dC_t = sum_d e h;  dB_t = sum_d G delta x;  dx = delta sum_s G B + D e;  d delta = sum_s G (A u + x B);  dA = sum_t G delta u;
 //     dD = sum_t e x;  dz = dy (C . h + D x) silu'(z);  dh_0 = exp(delta_1 A) G_1.
-// Tiles of 64 tokens, the last first, each from the state that the forward pass left at its first token.  A wave scans its eight tokens forwards and backwards
-// from zero; both chains over the waves' pieces run at once, four waves each; then it walks them again with what enters, states and decays in registers.
+// Tiles of 64 or 32 tokens, the last first, each from the state that the forward pass left at its first token.  A wave scans its eight tokens forwards and backwards
+// from zero; both chains over the waves' pieces run at once, four waves each (of four waves: one behind the other); then it walks them again with what enters, states and decays in registers.
 //
 // What bounds it: the vector ALU, some 26 issue slots a state and token, of which four are the exponential and four the sums over channels for dB and dC.
 #include "column_sums.cuh"
@@ -27,7 +27,7 @@ template <typename T, int LPC, int TOK, int W, bool VEC>
 __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
     using Lane = ScanLane<LPC, TOK>;
     constexpr int CHN = Lane::CHN, V = Lane::V, TILE = W * TOK, PITCH = ss_pitch(TOK);
-    static_assert(W >= 8 && TILE % SS_CKPT == 0, "a thread a state for either chain; a tile begins where a state is left");
+    static_assert(W == 4 || W == 8, "a thread a state for either chain, or for both");
     // a wave's own: its arrays lie at fixed distances, so that a lane holds one address for all of them
     struct Mine { f32x4 B[TOK * LPC], C[TOK * LPC]; float d[CHN * PITCH], x[CHN * PITCH], e[CHN * PITCH], y[CHN * PITCH]; };
     struct Meet { f32x4 P[W][64], E[W][64], G[W][64]; };
@@ -50,9 +50,9 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
         D[i] = p.D && i < L.carried ? ld_param(p.D, p.D_f32, L.dv + i) : 0.f;
         dD[i] = dbias[i] = 0.f;
     }
-    // a thread a state: the first four waves chain the states, the other four their gradients
+    // a thread a state: the first four waves chain the states, the other four (if there are) their gradients
     const int e = tid & 255, ec = (e >> 2) / LPC, es = 4 * ((e >> 2) % LPC) + (e & 3);
-    const bool forwards = tid < 256, backwards = tid >= 256 && tid < 512, there = (block % p.per_group) * CHN + ec < p.DD / p.G && es < p.S;
+    const bool forwards = tid < 256, backwards = W < 8 || tid >= 256, there = (block % p.per_group) * CHN + ec < p.DD / p.G && es < p.S;
 
     for (int unit = slot; unit < p.units; unit += p.slots) {
         const Unit U(p, unit);
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
         request((tiles - 1) * TILE + w * TOK);
         for (int tile = tiles - 1; tile >= until; --tile) {
             const int t0 = tile * TILE + w * TOK, tokens = min(max(len - t0, 0), TOK);
-            const float left = forwards ? p.ckpt[((ckpt_slot(p, n, bos) + tile * (TILE / SS_CKPT)) * p.blocks + block) * 256 + e] : 0.f;
+            const float left = forwards ? p.ckpt[((ckpt_slot(p, n, bos) + tile) * p.blocks + block) * 256 + e] : 0.f;
             float x[V], z[V], dy[V], v[V], ev[V], gz[V], delta[V], ee[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) { x[i] = rx[i]; z[i] = rz[i]; dy[i] = rdy[i]; v[i] = rdt[i] + bias[i]; }
@@ -157,23 +157,29 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
             meet.E[w][l] = E;
             meet.G[w][l] = G;
             __syncthreads();
-            if (tid < 512) {
-                float* const ends_at = reinterpret_cast<float*>(forwards ? meet.E : meet.G) + e;
+            {
                 const float* const f = reinterpret_cast<const float*>(meet.P) + e;
-                float ends[W], decays[W];
+                float decays[W], ends[W];
 #pragma unroll
-                for (int i = 0; i < W; ++i) { ends[i] = ends_at[i * 256]; decays[i] = f[i * 256]; }
+                for (int i = 0; i < W; ++i) decays[i] = f[i * 256];
                 if (forwards) {
-                    enters = left;
+                    float* const at = reinterpret_cast<float*>(meet.E) + e;
+                    float h = left;
+#pragma unroll
+                    for (int i = 0; i < W; ++i) ends[i] = at[i * 256];
 #pragma unroll
                     for (int i = 0; i < W; ++i) {
-                        ends_at[i * 256] = enters;
-                        enters = __builtin_fmaf(decays[i], enters, ends[i]);
+                        at[i * 256] = h;
+                        h = __builtin_fmaf(decays[i], h, ends[i]);
                     }
-                } else {
+                }
+                if (backwards) {
+                    float* const at = reinterpret_cast<float*>(meet.G) + e;
+#pragma unroll
+                    for (int i = 0; i < W; ++i) ends[i] = at[i * 256];
 #pragma unroll
                     for (int i = W - 1; i >= 0; --i) {
-                        ends_at[i * 256] = enters;
+                        at[i * 256] = enters;
                         enters = __builtin_fmaf(decays[i], enters, ends[i]);
                     }
                 }
@@ -288,12 +294,13 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
         if (l < CHN / V) { my.d[L.ch + i] = dD[i]; my.x[L.ch + i] = dbias[i]; }
     }
     __syncthreads();
-    if (tid < 256) {
+    if (forwards) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < W; ++i) s += reinterpret_cast<const float*>(meet.E)[i * 256 + e];
         if (there) p.part_own[(long long)slot * p.DD * (p.S + 2) + (long long)(L.d0 + ec) * p.S + es] = s;
-    } else if (backwards && e < CHN && (block % p.per_group) * CHN + e < p.DD / p.G) {
+    }
+    if (backwards && e < CHN && (block % p.per_group) * CHN + e < p.DD / p.G) {
         float s = 0.f, b = 0.f;
 #pragma unroll
         for (int i = 0; i < W; ++i) { s += mine[i].d[e]; b += mine[i].x[e]; }
@@ -312,11 +319,16 @@ static int grad_slots(const ScanPlan& s) {
 static size_t bc_bytes(const hdla_scan_dims* d, const ScanPlan& s) { return ((size_t)s.per_group * 2 * s.rows * d->G * d->S * 4 + 15) / 16 * 16; }
 static size_t own_bytes(const hdla_scan_dims* d, int slots) { return ((size_t)slots * d->D * (d->S + 2) * 4 + 15) / 16 * 16; }
 static size_t grad_bytes(const hdla_scan_dims* d, const ScanPlan& s, int slots) { return bc_bytes(d, s) + own_bytes(d, slots) + ends_bytes(s); }
-template <typename T, int LPC> static void launch_grad(const ScanArgs& a, bool vec, hipStream_t s) {
-    constexpr int TOK = SS_TOK, W = 8;
+template <typename T, int LPC, int W> static void launch_grad_waves(const ScanArgs& a, bool vec, hipStream_t s) {
+    constexpr int TOK = SS_TOK;
     const dim3 grid((unsigned)scan_workgroups(a.blocks, a.slots)), block(64 * W);
     if (vec) hipLaunchKernelGGL((scan_grad_kernel<T, LPC, TOK, W, true>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((scan_grad_kernel<T, LPC, TOK, W, false>), grid, block, 0, s, a);
+}
+template <typename T, int LPC> static void launch_grad(const ScanArgs& a, bool vec, hipStream_t s) {
+    static_assert(SS_TILE_MANY == 4 * SS_TOK && SS_TILE_FEW == 8 * SS_TOK, "a tile begins where a state is left");
+    if (a.every == SS_TILE_MANY) launch_grad_waves<T, LPC, 4>(a, vec, s);
+    else launch_grad_waves<T, LPC, 8>(a, vec, s);
 }
 template <typename T> static hipError_t launch_scan_grad(const ScanArgs& a, const ScanPlan& s, hipStream_t st) {
     switch (s.lpc) {

@@ -284,7 +284,8 @@ def _common(x, *others):
 
 
 class StateSpaceScanFunction(torch.autograd.Function):
-    """What is kept between the passes: the inputs, and the state that enters every 64th token (fp32: 1 / 64 of S numbers a channel and token)."""
+    """What is kept between the passes: the inputs, and the state that enters every 64th token (32nd where there are many sequences and
+    channels), fp32."""
 
     @staticmethod
     @autocast_custom_fwd

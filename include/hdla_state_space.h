@@ -39,7 +39,7 @@ int hdla_short_conv_step(const hdla_conv_dims* dims, const void* x, const void* 
  * x, dt, z [B, T, D] and B, C [B, T, G, S] of `dtype`, at any address and with strides of their own (elements; the last one is 1); A [D, S], D [D], dt_bias [D]
  * contiguous, each bf16 or fp32; D, z, dt_bias may be NULL.  States [N, D, S] fp32.  y, dy and the gradients are contiguous, 16-byte aligned.
  * cu_seqlens (device int64[N + 1], B = 1): packed sequences; rows of no sequence become zero in y and in the gradients.
- * hdla_scan_fwd: h0 and ht may be NULL.  states (hdla_scan_states_bytes() bytes, 16-byte aligned, or NULL): the state that enters every 64th token, for hdla_scan_bwd;
+ * hdla_scan_fwd: h0 and ht may be NULL.  states (hdla_scan_states_bytes() bytes, 16-byte aligned, or NULL): the state that enters every 64th token (32nd where there are many sequences and channels), for hdla_scan_bwd;
  * workspace of hdla_scan_fwd_workspace_bytes() bytes (0 where there are no segments), 16-byte aligned.
  * hdla_scan_bwd: dht, dh0, dD, ddt_bias, dz NULL where there is none (dh0 NULL: not wanted).  dx, ddt, dz [B, T, D], dB, dC [B, T, G, S] of `dtype`,
  * dA, dD, ddt_bias in the type of A, D, dt_bias.  Sums are taken in a fixed order through `workspace` (hdla_scan_workspace_bytes() bytes, 16-byte aligned).

@@ -65,6 +65,21 @@ def test_long_sequences_of_few_channels(nb, T, d, S, G, state, dtype):
     compare(low, ref, dy, dh, True)
 
 
+@pytest.mark.parametrize("nb,T,d,S,G,dtype", [(130, 35, 64, 16, 1, torch.bfloat16), (130, 33, 31, 8, 1, torch.float32), (20, 3, 2048, 16, 1, torch.bfloat16),
+                                              (65, 40, 64, 30, 2, torch.bfloat16), (140, 9, 15, 64, 1, torch.float32)])
+def test_many_sequences(nb, T, d, S, G, dtype):
+    """More workgroups than compute units; more sequences than workgroups side by side."""
+    low, ref, dy, dh = make(nb + T, nb, T, d, S, G, dtype)
+    compare(low, ref, dy, dh, True)
+
+
+def test_many_packed_sequences_of_few_tokens():
+    cu = torch.arange(0, 1042, 2)
+    cu[100:110] = cu[100]                                                    # (some of them empty)
+    low, ref, dy, dh = make(25, 1, 1040, 16, 16, 1, torch.bfloat16, N=len(cu) - 1)
+    compare(low, ref, dy, dh, True, cu)
+
+
 @pytest.mark.parametrize("inner", [(3, 700, 701), (256, 512, 1024), (1400, 1499, 1500), (0, 0, 1)])
 def test_long_packed_sequences_of_few_channels(inner):
     T = 1501
