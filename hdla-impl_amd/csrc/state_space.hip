@@ -284,7 +284,7 @@ extern "C" int hdla_scan_fwd(const hdla_scan_dims* dims, const void* x, const vo
     ScanPlan s;
     const int rc = scan_plan(dims, s);
     if (rc) return rc;
-    if (s.rows > 0 && (!x || !dt || !A || !B || !C || !y)) return HDLA_ERR_NULL;
+    if (!A || (s.rows > 0 && (!x || !dt || !B || !C || !y))) return HDLA_ERR_NULL;
     if (!fits(y, 16) || !fits(h0, 16) || !fits(ht, 16)) return HDLA_ERR_ALIGN;
     if (states && (!fits(states, 16) || states_bytes < (size_t)s.ckpt * s.blocks * 1024)) return HDLA_ERR_WORKSPACE;
     scan_segments(dims, s, SEGMENT_COST_FORWARD);

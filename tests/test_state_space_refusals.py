@@ -115,6 +115,7 @@ def test_c_entry_points_answer_wrong_dimensions_with_codes():
         assert lib.hdla_scan_bwd(by(d), *[None] * 11, 0, *[None] * 10, 0, None) == rc
         assert lib.hdla_scan_step(by(d), *[None] * 12) == rc
     assert lib.hdla_scan_step(by(_lib.HdlaScanDims(**scan)), *[None] * 12) == -2              # one token
+    assert lib.hdla_scan_fwd(by(_lib.HdlaScanDims(**dict(scan, T=0))), *[None] * 12, 0, None, 0, None) == -1      # A is read where there are no tokens, too
     norm = dict(rows=4, E=8, dtype=0, residual_dtype=0, weight_dtype=1, post_dtype=1, scale_dtype=1, act=1, post_norm=1, factor=1.0, eps=1e-5)
     assert lib.hdla_block_norm_workspace_bytes(by(_lib.HdlaBlockNormDims(**norm))) > 0
     for wrong, rc in ((dict(E=4097), -2), (dict(E=0), -2), (dict(act=3), -2), (dict(dtype=1), -4), (dict(rows=-1), -2), (dict(eps=float("nan")), -2)):
