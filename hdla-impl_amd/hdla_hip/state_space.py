@@ -19,7 +19,7 @@ from .utils import autocast_custom_bwd, autocast_custom_fwd
 
 _NATIVE = (torch.bfloat16, torch.float32)
 CONV_WIDTHS, MAX_STATES = (2, 3, 4), 64
-ROW_MOST = 1 << 24
+ROW_MOST, TOKENS_MOST, COUNT_MOST = 1 << 24, 1 << 30, (1 << 31) - 1
 
 
 def on_one_gpu(x, *others):
@@ -71,6 +71,13 @@ def _sequences(x, cu_seqlens, state, what):
     if state is not None and tuple(state.shape) != (n,) + what:
         raise ValueError(f"initial_state must be {(n,) + what}, one for each sequence, got {tuple(state.shape)}")
     return n, cu_seqlens
+
+
+def _within_reach(x, n):
+    """The kernels count rows and sequences in 32 bits."""
+    tokens = x.shape[1] if x.dim() == 3 else 1
+    if tokens > TOKENS_MOST or x.shape[0] * tokens > COUNT_MOST or n > COUNT_MOST or x.shape[-1] > ROW_MOST:
+        raise NotImplementedError(f"x {tuple(x.shape)} of {n} sequences is not built: at most 2^30 tokens a sequence, 2^31 - 1 tokens and sequences, 2^24 channels")
 
 
 def _not_trained(name):
@@ -160,6 +167,7 @@ def short_conv(
         raise ValueError(f"x must be [B, T, D], got {tuple(x.shape)}")
     silu = _conv_args(x, weight, bias, activation)
     n, cu = _sequences(x, cu_seqlens, initial_state, (weight.shape[1] - 1, x.shape[-1]))
+    _within_reach(x, n)
     on_one_gpu(x, weight, bias, initial_state)
     out_dtype = x.dtype
     if out_dtype == torch.float16:
@@ -222,6 +230,7 @@ def short_conv_step(
     silu = _conv_args(x, weight, bias, activation)
     if tuple(state.shape) != (x.shape[0], weight.shape[1] - 1, x.shape[1]):
         raise ValueError(f"state must be {(x.shape[0], weight.shape[1] - 1, x.shape[1])}, got {tuple(state.shape)}")
+    _within_reach(x, x.shape[0])
     on_one_gpu(x, state, weight, bias)
     out_dtype = x.dtype
     if out_dtype not in _NATIVE + (torch.float16,):
@@ -358,6 +367,7 @@ def state_space_scan(
         raise ValueError(f"x must be [B, T, D], got {tuple(x.shape)}")
     B, C = _scan_args(x, dt, A, B, C, D, z, dt_bias)
     n, cu = _sequences(x, cu_seqlens, initial_state, tuple(A.shape))
+    _within_reach(x, n)
     on_one_gpu(x, dt, A, B, C, D, z, dt_bias, initial_state)
     out_dtype = x.dtype
     x, dt, B, C, z = (rows(t) for t in _common(x, dt, B, C, z))
@@ -392,6 +402,7 @@ def state_space_step(
     B, C = _scan_args(x, dt, A, B, C, D, z, dt_bias)
     if tuple(state.shape) != (x.shape[0],) + tuple(A.shape):
         raise ValueError(f"state must be {(x.shape[0],) + tuple(A.shape)}, got {tuple(state.shape)}")
+    _within_reach(x, x.shape[0])
     on_one_gpu(x, dt, A, B, C, state, D, z, dt_bias)
     out_dtype, to = x.dtype, _new_state(state, inplace, torch.float32)
 

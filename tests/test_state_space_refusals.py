@@ -84,6 +84,22 @@ def test_state_space_step(kw, error, match):
         state_space_step(**args)
 
 
+def test_sizes_that_32_bits_do_not_hold():
+    one, many = torch.zeros(1), 2 ** 31
+    for shape in ((1, many, 8), (1, 2 ** 32 + 4, 8), (3, 2 ** 30, 8), (many, 1, 8), (1, 2, 2 ** 24 + 8)):
+        x, S = one.expand(shape), one.expand(shape[:2] + (4,))
+        with pytest.raises(NotImplementedError, match="is not built"):
+            short_conv(x, one.expand(shape[-1], 4))
+        with pytest.raises(NotImplementedError, match="is not built"):
+            state_space_scan(x, x, one.expand(shape[-1], 4), S, S)
+    for shape in ((many, 8), (2 ** 32 + 1, 8), (2, 2 ** 24 + 8)):
+        x, S = one.expand(shape), one.expand(shape[0], 4)
+        with pytest.raises(NotImplementedError, match="is not built"):
+            short_conv_step(x, one.expand(shape[0], 3, shape[1]), one.expand(shape[1], 4))
+        with pytest.raises(NotImplementedError, match="is not built"):
+            state_space_step(x, x, one.expand(shape[1], 4), S, S, one.expand(shape + (4,)))
+
+
 @pytest.mark.parametrize("kw,error,match", [
     (dict(x=r(3, 4097), residual=None), NotImplementedError, "4097 channels"), (dict(residual=r(3, 7)), ValueError, "residual"), (dict(gate=r(8)), ValueError, "gate"),
     (dict(weight=r(3, 8)), ValueError, "weight must be"), (dict(post_weight=r(7)), ValueError, "post_weight"), (dict(residual_scale=r(1)), ValueError, "residual_scale"),
