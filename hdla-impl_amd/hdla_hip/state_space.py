@@ -201,6 +201,12 @@ def _run_step(name, fn, tensors, inplace):
     return fn(*tensors)
 
 
+def _written(state):
+    """A state that a kernel has written in place: a graph that kept it notices, as with torch's own operations."""
+    if state is not None and not state.is_inference():
+        torch.autograd.graph.increment_version(state)
+
+
 def _new_state(state, inplace, dtype):
     """Where the next state goes: the state's own place, which has to be as the kernels want it."""
     if not inplace:
@@ -246,6 +252,7 @@ def short_conv_step(
             y, new = torch.empty(x.shape, dtype=own, device=x.device), torch.empty_like(s) if to is None else to
             _lib.check(_lib.load().hdla_short_conv_step(ctypes.byref(dims), _lib.ptr(xs), _lib.ptr(w), _lib.ptr(b), _lib.ptr(s), _lib.ptr(y), _lib.ptr(new),
                                                         _lib.current_stream(x.device)), "hdla_short_conv_step")
+            _written(to)
         return y.to(out_dtype), new if to is not None else new.to(out_dtype)
 
     return _run_step("short_conv_step", call, (x, state, weight, bias), inplace)
@@ -311,8 +318,8 @@ class StateSpaceScanFunction(torch.autograd.Function):
             _lib.check(lib.hdla_scan_fwd(ctypes.byref(dims), _lib.ptr(x), _lib.ptr(dt), _lib.ptr(A), _lib.ptr(B), _lib.ptr(C), _lib.ptr(D), _lib.ptr(z), _lib.ptr(bias),
                                          _lib.ptr(h0), _lib.ptr(y), _lib.ptr(ht), _lib.ptr(left), 0 if left is None else left.numel(), _lib.ptr(ws), ws.numel(),
                                          _lib.current_stream(x.device)), "hdla_scan_fwd")
-        ctx.save_for_backward(x, dt, A, B, C, D, z, bias, h0, cu, left)
-        ctx.cfg = (softplus, n)
+        ctx.save_for_backward(x, dt, A, B, C, D, z, bias, cu, left)      # (the initial state's part in them is in `left`)
+        ctx.cfg = (softplus, n, h0 is not None)
         ctx.set_materialize_grads(False)
         return y, ht
 
@@ -320,15 +327,16 @@ class StateSpaceScanFunction(torch.autograd.Function):
     @once_differentiable
     @autocast_custom_bwd
     def backward(ctx, dy, dht):
-        x, dt, A, B, C, D, z, bias, h0, cu, left = ctx.saved_tensors
-        softplus, n = ctx.cfg
+        x, dt, A, B, C, D, z, bias, cu, left = ctx.saved_tensors
+        softplus, n, want_dh0 = ctx.cfg
         lib = _lib.load()
         new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
         with torch.cuda.device(x.device):
             dims = _scan_dims(x, dt, A, B, C, D, z, bias, softplus, n, cu)
             dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else whole(dy.to(x.dtype))
             dht = None if dht is None else whole(dht.float())
-            dx, ddt, dA, dB, dC, dD, dz, dbias, dh0 = (new(t) for t in (x, dt, A, B, C, D, z, bias, h0))
+            dx, ddt, dA, dB, dC, dD, dz, dbias = (new(t) for t in (x, dt, A, B, C, D, z, bias))
+            dh0 = torch.empty(n, x.shape[-1], A.shape[1], dtype=torch.float32, device=x.device) if want_dh0 else None
             ws = torch.empty(lib.hdla_scan_workspace_bytes(ctypes.byref(dims)), dtype=torch.uint8, device=x.device)
             _lib.check(lib.hdla_scan_bwd(ctypes.byref(dims), _lib.ptr(x), _lib.ptr(dt), _lib.ptr(A), _lib.ptr(B), _lib.ptr(C), _lib.ptr(D), _lib.ptr(z), _lib.ptr(bias),
                                          _lib.ptr(dy), _lib.ptr(dht), _lib.ptr(left), left.numel(), _lib.ptr(dx), _lib.ptr(ddt), _lib.ptr(dA), _lib.ptr(dB),
@@ -415,6 +423,7 @@ def state_space_step(
             y, new = torch.empty(x.shape, dtype=xs.dtype, device=x.device), torch.empty_like(s) if to is None else to
             _lib.check(_lib.load().hdla_scan_step(ctypes.byref(dims), _lib.ptr(xs), _lib.ptr(dts), _lib.ptr(A), _lib.ptr(Bs), _lib.ptr(Cs), _lib.ptr(D), _lib.ptr(zs),
                                                   _lib.ptr(dt_bias), _lib.ptr(s), _lib.ptr(y), _lib.ptr(new), _lib.current_stream(x.device)), "hdla_scan_step")
+            _written(to)
         return y.to(out_dtype), new
 
     return _run_step("state_space_step", call, (x, dt, A, B, C, state, D, z, dt_bias), inplace)

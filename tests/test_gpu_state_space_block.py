@@ -224,3 +224,31 @@ def test_calls_on_two_streams_do_not_meet():
         torch.cuda.synchronize()
     for y, r, left in outs:
         assert torch.equal(y, want[0]) and torch.equal(r, want[1]) and torch.equal(left["scan"], want[2]["scan"])
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_state_that_a_graph_keeps_is_not_written_over_unnoticed(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(_lib, "_native", _lib._NoNative())
+    g = torch.Generator().manual_seed(5)
+    rn = lambda *s: torch.randn(*s, generator=g).to(DEV)
+    x, w, A, B = rn(2, 9, 16).requires_grad_(), rn(16, 4), -torch.exp(rn(16, 8)), rn(2, 9, 8)
+    near, far = rn(2, 3, 16), rn(2, 16, 8)
+    y, _ = short_conv(x, w, initial_state=near)
+    short_conv_step(rn(2, 16), near, w, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    out = []
+    for write in (False, True):                           # (of the scan's state the backward pass needs nothing)
+        v = x.detach().requires_grad_()
+        y, _ = state_space_scan(v, v, A, B, B, dt_softplus=True, initial_state=far)
+        if write:
+            before = far._version
+            state_space_step(rn(2, 16), rn(2, 16), A, B[:, 0], B[:, 0], far, inplace=True)
+            assert far._version > before
+        out.append(torch.autograd.grad(y.sum(), v)[0])
+    assert torch.equal(*out)
+    with torch.inference_mode():                          # (whose tensors no graph keeps)
+        near = rn(2, 3, 16)
+        short_conv_step(rn(2, 16), near, w, inplace=True)
+    torch.cuda.synchronize()
