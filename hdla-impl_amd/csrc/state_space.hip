@@ -34,7 +34,7 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
     f32x4 A2 = zero4();
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (j < L.left) A2[j] = ld_param(p.A, p.A_f32, (long long)L.d * p.S + 4 * L.q + j) * LOG2E;
+        if (j < L.left) A2[j] = ld_decay(p.A, p.A_f32, (long long)L.d * p.S + 4 * L.q + j);
     if (tid < CHN) {
         const bool in = (block % p.per_group) * CHN + tid < p.DD / p.G;
         bias[tid] = p.bias && in ? ld_param(p.bias, p.bias_f32, L.d0 + tid) : 0.f;

@@ -28,7 +28,7 @@ __global__ __launch_bounds__(512) void scan_ends_kernel(ScanArgs p) {
     float bias[V], sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (j < L.left) A2[j] = ld_param(p.A, p.A_f32, (long long)L.d * p.S + 4 * L.q + j) * LOG2E;
+        if (j < L.left) A2[j] = ld_decay(p.A, p.A_f32, (long long)L.d * p.S + 4 * L.q + j);
 #pragma unroll
     for (int i = 0; i < V; ++i) bias[i] = p.bias && i < L.carried ? ld_param(p.bias, p.bias_f32, L.dv + i) : 0.f;
     const int pieces = (U.to - U.from + W * TOK - 1) / (W * TOK), start = U.from + w * pieces * TOK, begin = BACK ? start + (pieces - 1) * TOK : start;

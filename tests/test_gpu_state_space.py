@@ -217,6 +217,23 @@ def test_extreme_step_sizes():
     compare(low, ref, dy, dh, True)
 
 
+@pytest.mark.parametrize("d,T", [(20, 11), (20, 100), (8, 3001)])
+def test_states_that_decay_at_once(d, T):
+    # A = -inf: a state is what its last token adds
+    low, ref, dy, dh = make(41 + T, 1, T, d, 8, 1, torch.float32)
+    low["A"][:, ::3] = ref["A"].data[:, ::3] = -float("inf")
+    v = put(low)
+    y, ht = call(v, True)
+    yr, hr = O.scan(*[ref[k].detach() for k in NAMES[:8]], True, ref["h0"].detach())
+    finite = {k: t.detach().clone() for k, t in ref.items()}
+    finite["A"][:, ::3] = -1e30
+    m, count = O.scan_magnitudes(*[finite[k].requires_grad_() for k in NAMES[:8]], True, finite["h0"].requires_grad_(), None, dy.double(), dh.double())
+    close("y", y, yr, m["y"], count)
+    close("ht", ht, hr, m["ht"], count)
+    grads = torch.autograd.grad([y, ht], list(v.values()), [dy.to(DEV), dh.to(DEV)])
+    assert all(torch.isfinite(t).all() for t in grads) and (grads[2][:, ::3] == 0).all() and (grads[8][:, :, ::3] == 0).all()
+
+
 def test_inputs_that_are_not_finite_stay_in_their_channel_and_sequence():
     low, _, _, _ = make(16, 2, 70, 16, 16, 1, torch.float32)
     clean, _ = call(put(low, False), True)
