@@ -7,6 +7,7 @@
 //
 // Streams through HBM: forward reads x, gate, residual and writes y, r; backward reads these, dy, dr and writes dx, dgate, dresidual.  A row lies in the registers
 // of one wave, or of two, four or eight waves of a workgroup where it is long, 16 bytes a lane and piece; its sums are taken across lanes without LDS (several waves' through it).
+// 16384 x 4096 in bf16 with an fp32 stream: forward 177 us, 5.3 TB/s, what a large copy reaches; 8192 x 2048 in bf16 forward 28 us, backward 58, the sums of the weights' gradients 9.
 // Workgroups stride over rows: weights are read once, and the gradients of weights and scale stay in registers until a workgroup leaves one row of partial sums.
 #include "column_sums.cuh"
 #include "hdla_common.cuh"
@@ -360,10 +361,12 @@ static int block_norm_config(const hdla_block_norm_dims* d, bool bwd, BlockNormC
     if (d->rows < 0 || d->rows > (1LL << 40) || d->E < 1 || !(d->eps >= 0.f) || d->act < ACT_NONE || d->act > ACT_SILU) return HDLA_ERR_SHAPE;
     if (d->E > BLOCK_NORM_MOST) return HDLA_ERR_SHAPE;
     const int n = d->dtype == HDLA_BF16 ? 8 : 4, pieces = (d->E + n - 1) / n;
+    // one piece a lane, up to 512 lanes; two pieces of half as many lanes are alike (8192 x 4096 in bf16, forward and backward 205 us; so 201)
     c.waves = pieces <= 64 ? 1 : pieces <= 128 ? 2 : pieces <= 256 || (pieces <= 512 && n == 4) ? 4 : 8;
     c.nv = pieces > 64 * c.waves ? 2 : 1;
     const long long per = c.waves >= 4 ? 1 : 4 / c.waves, need = (d->rows + per - 1) / per, most = bwd ? BLOCK_NORM_GRAD_WGS : BLOCK_NORM_WGS;
-    // as many as are resident, with as many rows each as the others
+    // as many as are resident, with as many rows each as the others.  us, forward and backward, of 512 / 768 / 1024 workgroups backward (forward 1024, 2048 and 4096 are alike):
+    // 8192 x 2048 in bf16 107 / 96 / 106, 16384 x 1024 103 / 87 / 92, 16384 x 4096 491 / 490 / 487
     const long long turns = (need + most - 1) / most;
     c.wgs = std::max(1LL, turns ? (need + turns - 1) / turns : 1);
     c.vec = d->E % n == 0;

@@ -26,9 +26,9 @@ struct ConvArgs {
 };
 
 // V channels of W taps, [V][W] as they lie
-template <int W, int V> __device__ __forceinline__ void ld_taps(const void* w, int f32, long long at, float (&t)[V][W], bool whole) {
+template <int W, int V> __device__ __forceinline__ void ld_taps(const void* w, int f32, long long at, float (&t)[V][W]) {
     constexpr int N = V * W;
-    if (whole && V > 1) {
+    if constexpr (V > 1) {
         if (f32) {
 #pragma unroll
             for (int i = 0; i < N; i += 4) {
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256) void short_conv_kernel(ConvArgs p, int steps) 
 #pragma unroll
     for (int i = 0; i < STEP; ++i) row(t0 + i, now[i]);
     float w[V][W], b[V];
-    ld_taps<W, V>(p.weight, p.w_f32, (long long)col * W, w, true);
+    ld_taps<W, V>(p.weight, p.w_f32, (long long)col * W, w);
 #pragma unroll
     for (int k = 0; k < V; ++k) b[k] = p.bias ? ld_param(p.bias, p.b_f32, col + k) : 0.f;
     // (before a packed batch's first token nothing is read: these rows are of another sequence, or of none)
@@ -220,7 +220,7 @@ template <typename T, int W, int V> __device__ __forceinline__ void conv_dstate(
     if (p.cu) packed_bounds(p.cu, (int)n, p.T, bos, eos);
     const int64_t len = eos - bos, row0 = p.cu ? bos : n * p.T;
     float w[V][W], b[V], d[V];
-    ld_taps<W, V>(p.weight, p.w_f32, (long long)col * W, w, true);
+    ld_taps<W, V>(p.weight, p.w_f32, (long long)col * W, w);
 #pragma unroll
     for (int k = 0; k < V; ++k) { b[k] = p.bias ? ld_param(p.bias, p.b_f32, col + k) : 0.f; d[k] = 0.f; }
     // token t's tap j meets row t + j of [state, tokens]
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(256) void short_conv_grad_kernel(ConvArgs p, int st
 #pragma unroll
         for (int i = 0; i < STEP; ++i) rows(first + i, x[i], dy[i]);
         float w[V][W], b[V], ring[W][V];                  // ring: g of the last W tokens
-        ld_taps<W, V>(p.weight, p.w_f32, (long long)col * W, w, true);
+        ld_taps<W, V>(p.weight, p.w_f32, (long long)col * W, w);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             b[k] = p.bias ? ld_param(p.bias, p.b_f32, col + k) : 0.f;
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(256) void short_conv_step_kernel(ConvArgs p) {
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) x[j].load(static_cast<const T*>(p.state) + (n * (W - 1) + j) * p.D + col, V);
     x[W - 1].load(static_cast<const T*>(p.x.p) + n * p.x.batch + col, V);
-    ld_taps<W, V>(p.weight, p.w_f32, (long long)col * W, w, true);
+    ld_taps<W, V>(p.weight, p.w_f32, (long long)col * W, w);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
         f[k] = p.bias ? ld_param(p.bias, p.b_f32, col + k) : 0.f;
@@ -581,6 +581,7 @@ extern "C" int hdla_short_conv_bwd(const hdla_conv_dims* dims, const void* x, co
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const ConvGradPlan g = conv_grad_plan(dims);
     hipError_t e;
+    // four channels a thread also in bf16: eight need the registers of twice as many sums (8192 x 2048, forward and backward 69 us; so 56)
     if (dims->dtype == HDLA_BF16) e = conv_vec(dims, 4, a) ? launch_conv_grad<bf16, 4>(a, dims->W, g, s) : launch_conv_grad<bf16, 1>(a, dims->W, g, s);
     else e = conv_vec(dims, 4, a) ? launch_conv_grad<float, 4>(a, dims->W, g, s) : launch_conv_grad<float, 1>(a, dims->W, g, s);
     if (e != hipSuccess) return (int)e;

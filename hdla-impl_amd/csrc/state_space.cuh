@@ -5,8 +5,8 @@
 //
 // Lanes: LPC lanes of a wave hold the states of one channel, four each, and a wave has 64 / LPC channels and L tokens at a time.  The W waves
 // of a workgroup take consecutive pieces of L tokens.  Every wave scans its piece from zero, the pieces' decays and ends meet in LDS, where one thread
-// a state chains them, and the wave walks its piece once more from the state that enters it.  The exponentials are formed once, four
-// issue slots each where a multiplication takes one, and stay in registers for the second walk: that one costs two slots a state.
+// a state chains them, and the wave walks its piece once more from the state that enters it.  The exponentials are formed once, two
+// issue slots each (8.1 cycles a wave where a multiplication takes 4.1), and stay in registers for the second walk: that one costs two slots a state.
 #pragma once
 #include "hdla_common.cuh"
 #include "row_tile.cuh"
@@ -68,7 +68,6 @@ template <int V> struct Raw<bf16, V, true> {
     uint32_t w[NW];
     __device__ __forceinline__ void load(const bf16* p, int) {
         if constexpr (V == 1) w[0] = p->x;
-        else if constexpr (V == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
         else if constexpr (V == 4) { const u32x2 r = *reinterpret_cast<const u32x2*>(p); w[0] = r[0]; w[1] = r[1]; }
         else { const u32x4 r = *reinterpret_cast<const u32x4*>(p); w[0] = r[0]; w[1] = r[1]; w[2] = r[2]; w[3] = r[3]; }
     }

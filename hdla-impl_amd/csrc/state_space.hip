@@ -1,7 +1,8 @@
 // The selective state space scan, forward (state_space.cuh has the formulas and how lanes and waves share the work), and its single-token step.
 //
-// What bounds the scan: the vector ALU.  A state and token cost one multiplication and one exponential (four issue slots) for the decay and six more
-// slots for the two walks, against 8 bytes of x, dt, z, y a channel and token of bf16.
+// What bounds the scan: the vector ALU, busy 88 to 90 % of the time (8192 x 4096 x 16 184 us, 4 x 2048 x 2048 x 16 75).  A state and token cost a multiplication and an exponential
+// (two issue slots) for the decay, two slots for the walk from zero and two for the other, against 8 bytes of x, dt, z, y a channel and token of bf16; the rest are step
+// sizes, gates and what brings operands into place.
 #include "hdla_launch.h"
 #include "state_space.cuh"
 #include "state_space_ends.h"
@@ -239,12 +240,14 @@ template <typename T, int LPC, int W, bool VEC> static void launch_tokens(const 
 }
 // Waves of a workgroup.  Where the registers of four waves a SIMD suffice: eight, two workgroups a compute unit, if there are as many; else sixteen.  Where they don't: twelve.
 // Short sequences: four.  us, eight / twelve / sixteen (and 16 tokens a wave, eight waves): 8192 x 4096 channels, 256 workgroups, 245 / 214 / 195 (215); 4 x 2048 x 2048, 512 of them,
-// 72 / 84 / 77 (94).
+// 72 / 84 / 77 (94).  Four / eight: 8 x 64 x 2048 11 / 14, 256 x 32 x 2048 156 / 303, 64 x 128 x 2048 100 / 122, but 4 x 128 x 1024, 256 workgroups, 10.2 / 8.5.
 template <typename T, int LPC, bool VEC> static void launch_lpc(const ScanArgs& a, hipStream_t s) {
     constexpr bool lean = LPC == 8 || (VEC && sizeof(T) == 2 && LPC >= 4);
-    if (a.T / (a.cu ? a.N : 1) <= 64) launch_tokens<T, LPC, 4, VEC>(a, s);
+    const int average = a.T / (a.cu ? a.N : 1);
+    const bool many = scan_workgroups(a.blocks, a.units) >= 512;
+    if (average <= 64 || (average <= 128 && many)) launch_tokens<T, LPC, 4, VEC>(a, s);
     else if constexpr (!lean) launch_tokens<T, LPC, 12, VEC>(a, s);
-    else if (scan_workgroups(a.blocks, a.units) >= 512) launch_tokens<T, LPC, 8, VEC>(a, s);
+    else if (many) launch_tokens<T, LPC, 8, VEC>(a, s);
     else launch_tokens<T, LPC, 16, VEC>(a, s);
 }
 template <typename T> static hipError_t launch_scan(const ScanArgs& a, const ScanPlan& s, hipStream_t st) {
@@ -318,9 +321,10 @@ extern "C" int hdla_scan_step(const hdla_scan_dims* dims, const void* x, const v
     a.h0 = state; a.ht = new_state; a.y = y;
     int log2 = 0;
     while ((4 << log2) < dims->S) ++log2;
-    // four sequences a thread where that leaves every compute unit eight waves
+    // four sequences a thread where that leaves every compute unit sixteen waves.  us, one / four, of 4096 channels with 16 states: 4 sequences 3.4 / 4.9, 32 of them (the half of
+    // that) 6.0 / 6.5, 64 9.1 / 9.1, 256 27.5 / 24.6
     const long long blocks = (((long long)a.DD << log2) + 255) / 256;
-    const int nb = blocks * ((a.N + 3) / 4) >= 512 ? 4 : 1;
+    const int nb = blocks * ((a.N + 3) / 4) >= 1024 ? 4 : 1;
     const long long rows = (a.N + nb - 1) / nb;
     if (blocks > 0x7fffffffLL || rows > 65535) return HDLA_ERR_SHAPE;
     const int es = dims->dtype == HDLA_BF16 ? 2 : 4;
