@@ -7,6 +7,7 @@ namespace hdla {
 
 struct ColumnSums {
     const float* part;
+    int phases;                       // (the launch's)
     long long columns, rows, apart;   // apart: elements from one row to the next (0: columns)
     int results;
     long long end[4];             // of each result's columns
@@ -26,6 +27,6 @@ struct ColumnSums {
         columns = at + n;
     }
 };
-hipError_t launch_column_sums(const ColumnSums& s, hipStream_t stream);
+hipError_t launch_column_sums(const ColumnSums& s, hipStream_t stream, const ColumnSums& more = ColumnSums{});
 
 }  // namespace hdla

@@ -3,12 +3,12 @@
 
 namespace hdla {
 
-// PH threads a column, each every PH-th row; their sums are added in order
-template <int PH> __global__ __launch_bounds__(256) void column_sums_kernel(ColumnSums s) {
-    constexpr int COLS = 256 / PH;
-    __shared__ float red[PH > 1 ? PH : 1][COLS];
-    const int c = threadIdx.x % COLS, ph = threadIdx.x / COLS;
-    const long long col = (long long)blockIdx.x * COLS + c;
+// `phases` threads a column, each every so many-th row; their sums are added in order.  Two lots of partial results in one launch: the workgroups from `first` on have the other's.
+__global__ __launch_bounds__(256) void column_sums_kernel(ColumnSums one, ColumnSums other, unsigned first) {
+    __shared__ float red[256];
+    const ColumnSums& s = blockIdx.x < first ? one : other;
+    const int cols = 256 / s.phases, c = threadIdx.x & (cols - 1), ph = threadIdx.x / cols;
+    const long long col = (long long)(blockIdx.x < first ? blockIdx.x : blockIdx.x - first) * cols + c;
     int decreases = 0;
     if (s.cu) {
         for (int n = threadIdx.x; n < s.N; n += 256) decreases |= s.cu[n + 1] < s.cu[n];
@@ -31,14 +31,13 @@ template <int PH> __global__ __launch_bounds__(256) void column_sums_kernel(Colu
     if (col < s.columns && covered) {
         const float* p = s.part + col;
 #pragma unroll 8
-        for (long long r = ph; r < s.rows; r += PH) sum += p[r * s.apart];
+        for (long long r = ph; r < s.rows; r += s.phases) sum += p[r * s.apart];
     }
-    if constexpr (PH > 1) {
-        red[ph][c] = sum;
+    if (s.phases > 1) {
+        red[threadIdx.x] = sum;
         __syncthreads();
         if (ph) return;
-#pragma unroll
-        for (int i = 1; i < PH; ++i) sum += red[i][c];
+        for (int i = 1; i < s.phases; ++i) sum += red[i * cols + c];
     }
     if (col >= s.columns) return;
     int at = 0;
@@ -49,16 +48,19 @@ template <int PH> __global__ __launch_bounds__(256) void column_sums_kernel(Colu
     else st_elem(static_cast<bf16*>(s.out[at]) + e, sum);
 }
 
-hipError_t launch_column_sums(const ColumnSums& sums, hipStream_t stream) {
-    ColumnSums s = sums;
-    if (!s.columns) return hipSuccess;
+// threads a column, and the workgroups
+static long long shares(ColumnSums& s) {
     if (!s.apart) s.apart = s.columns;
     // us, 1 / 16 threads a column: 745 rows of 6144 columns (a norm's weights) 36 / 9, 104 of 10240 (a convolution's) 5.2 / 4.0; 128 of 262144 (a scan's dB and dC) 22 with either
-    const int ph = s.rows < 8 || s.columns >= 65536 * 4 ? 1 : 16;
-    const long long blocks = (s.columns * ph + 255) / 256;
+    s.phases = s.rows < 8 || s.columns >= 65536 * 4 ? 1 : 16;
+    return (s.columns * s.phases + 255) / 256;
+}
+hipError_t launch_column_sums(const ColumnSums& sums, hipStream_t stream, const ColumnSums& more) {
+    ColumnSums one = sums, other = more;
+    const long long first = shares(one), blocks = first + shares(other);
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    if (ph == 1) hipLaunchKernelGGL(column_sums_kernel<1>, dim3((unsigned)blocks), dim3(256), 0, stream, s);
-    else hipLaunchKernelGGL(column_sums_kernel<16>, dim3((unsigned)blocks), dim3(256), 0, stream, s);
+    if (!blocks) return hipSuccess;
+    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, one, other, (unsigned)first);
     return hipGetLastError();
 }
 

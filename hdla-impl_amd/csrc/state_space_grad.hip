@@ -394,13 +394,11 @@ extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const vo
     c.cu = a.cu; c.N = a.N; c.T = a.T; c.per_token = inner; c.tokens_end = 2 * s.rows * inner;
     c.add(dB, es == 4, s.rows * inner);
     c.add(dC, es == 4, s.rows * inner);
-    e = launch_column_sums(c, st);
-    if (e != hipSuccess) return (int)e;
     ColumnSums k{};
     k.part = a.part_own; k.rows = s.slots;
     k.add(dA, a.A_f32, (long long)dims->D * dims->S);
     k.add(D ? dD : nullptr, a.D_f32, dims->D);
     k.add(dt_bias ? ddt_bias : nullptr, a.bias_f32, dims->D);
-    e = launch_column_sums(k, st);
+    e = launch_column_sums(c, st, k);
     return e == hipSuccess ? HDLA_OK : (int)e;
 }
