@@ -2,7 +2,7 @@
 // the state before its first one: G_t = exp(delta_t A) (G_{t+1} + C_t e_t), e_t = dy_t silu(z_t).
 //
 // A workgroup has a segment of a block of channels; each of its eight waves walks an eighth of the tokens by itself, and they meet once, at the end.  Bound by the vector ALU:
-// five issue slots a state and token, of the seven (from the back: of the 24) that the scan takes.
+// half of the issue slots a state and token that the scan takes, from the back a sixth.
 #include "state_space_ends.h"
 
 namespace hdla {
