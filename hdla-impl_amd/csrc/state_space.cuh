@@ -24,7 +24,7 @@ constexpr int ss_pitch(int L) { return L + 4; }
 constexpr int SS_TOK = 8;             // tokens of a wave at a time
 // Tokens between the states that a forward pass leaves for the backward pass: a tile of that pass, of four waves where there are workgroups for two on every compute unit,
 // whose barriers then fall into each other's work, else of eight.  us a training step, eight / four: 4 x 2048 x 2048 (512 workgroups of four waves) 432 / 416, 2503 x 520 in fp32 (264) 152 / 181.
-constexpr int SS_TILE_FEW = 64, SS_TILE_MANY = 32;
+constexpr int SS_TILE_FEW = 64, SS_TILE_MANY = 32;      // (2^6, 2^5)
 
 // element (b, t, .) of an operand: base + b batch + t row.  A wave's tokens are reached by 32-bit offsets from its first one's row.
 struct Operand {
@@ -47,7 +47,7 @@ struct ScanArgs {
     const int64_t* cu;
     int T, N, DD, S, G, softplus;
     int per_group, blocks;            // channel blocks of a group, of all of them
-    int every;                        // SS_TILE_FEW or SS_TILE_MANY
+    int every_log2;                   // of SS_TILE_FEW or SS_TILE_MANY
     // backward
     const void* dy;                   // [rows, D]
     const float* dht;
@@ -144,6 +144,10 @@ template <typename T, int V, bool VEC> __device__ __forceinline__ void st_values
     if constexpr (VEC && V == 8 && sizeof(T) == 2) {
         const s16x4 lo = to_frag<T>(f32x4{x[0], x[1], x[2], x[3]}).v, hi = to_frag<T>(f32x4{x[4], x[5], x[6], x[7]}).v;
         *reinterpret_cast<s16x8*>(p) = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else if constexpr (VEC && V == 2 && sizeof(T) == 2) {
+        *reinterpret_cast<uint32_t*>(p) = __builtin_bit_cast(u32x2, to_frag<T>(f32x4{x[0], x[1], 0.f, 0.f}).v)[0];
+    } else if constexpr (VEC && V == 2) {
+        *reinterpret_cast<u32x2*>(p) = u32x2{__float_as_uint(x[0]), __float_as_uint(x[1])};
     } else if constexpr (VEC && V % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < V; i += 4) st_frag(p + i, to_frag<T>(f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]}));
@@ -319,9 +323,10 @@ __device__ __forceinline__ void apart() { __builtin_amdgcn_sched_barrier(0); }
 // sums over the LPC lanes of a channel
 template <int LPC, int N> __device__ __forceinline__ void sum_channel(float (&x)[N]) { sum_lanes<N>(x, LPC); }
 
-// first slot of a sequence in the states that a forward pass leaves: packed sequences' counts are not known to the host, and these never overlap
-__device__ __forceinline__ long long ckpt_slot(const ScanArgs& p, int n, int64_t bos) {
-    return p.cu ? bos / p.every + n : (long long)n * ((p.T + p.every - 1) / p.every);
+// A block's states in the first slot of a sequence, of those that a forward pass leaves: packed sequences' counts of slots are not known to the host, and these never overlap
+__device__ __forceinline__ float* ckpt_of(const ScanArgs& p, int n, int64_t bos, int block) {
+    const long long slot = p.cu ? (bos >> p.every_log2) + n : (long long)n * ((p.T + (1 << p.every_log2) - 1) >> p.every_log2);
+    return p.ckpt + (slot * p.blocks + block) * 256;
 }
 inline long long ckpt_slots(bool packed, long long T, long long N, int every) {
     return packed ? T / every + N + 1 : N * ((T + every - 1) / every);
@@ -405,7 +410,7 @@ inline ScanArgs scan_args(const hdla_scan_dims* d, const ScanPlan& s, const void
     a.B_group = d->B_group; a.C_group = d->C_group;
     a.A_f32 = d->A_dtype == HDLA_FP32; a.D_f32 = d->D_dtype == HDLA_FP32; a.bias_f32 = d->bias_dtype == HDLA_FP32;
     a.cu = d->cu_seqlens; a.T = d->T; a.N = d->N; a.DD = d->D; a.S = d->S; a.G = d->G; a.softplus = d->softplus != 0;
-    a.per_group = s.per_group; a.blocks = s.blocks; a.every = s.every; a.rows = s.rows; a.slots = s.slots;
+    a.per_group = s.per_group; a.blocks = s.blocks; a.every_log2 = s.every == SS_TILE_MANY ? 5 : 6; a.rows = s.rows; a.slots = s.slots;
     a.seg = s.seg; a.units = (int)s.units;
     return a;
 }

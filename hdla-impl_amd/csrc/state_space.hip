@@ -53,6 +53,7 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
             enters = __builtin_fmaf(left[256], enters, left[0]);
         }
 
+    float* const ckpt = p.ckpt ? ckpt_of(p, n, bos, block) : nullptr;
     Raw<T, V, VEC> rx, rdt, rz;
     StatesOf<T, LPC, TOK, VEC> rB, rC;
     const long long first = bos + U.from + w * TOK;
@@ -136,8 +137,8 @@ __global__ __launch_bounds__(64 * W) void scan_tokens_kernel(ScanArgs p) {
         }
         __syncthreads();
         f32x4 h = meet.E[w][l];
-        if (p.ckpt && (t0 & (p.every - 1)) == 0 && tokens > 0)
-            *reinterpret_cast<f32x4*>(p.ckpt + (((ckpt_slot(p, n, bos) + t0 / p.every) * p.blocks + block) * 64 + l) * 4) = h;
+        if (ckpt && (t0 & ((1 << p.every_log2) - 1)) == 0 && tokens > 0)
+            *reinterpret_cast<f32x4*>(ckpt + (long long)(t0 >> p.every_log2) * p.blocks * 256 + l * 4) = h;
         float y[TOK];
         f32x4 cc = my.C[L.q];
 #pragma unroll

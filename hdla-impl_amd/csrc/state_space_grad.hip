@@ -91,10 +91,14 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
             rC.load(cC, (uint32_t)p.C.row, tokens, p.S);
             cx.next(); cdt.next(); cz.next(); cdy.next(); cB.next(); cC.next();
         };
+        const float* const entered = ckpt_of(p, n, bos, block);
+        // this block's part of dB and dC: [block of the group][B, C][row][group][S]
+        const long long inner = (long long)p.G * p.S, half = p.rows * inner;
+        float* const part0 = p.part_bc + 2 * half * (block % p.per_group) + (long long)L.group * p.S;
         request((tiles - 1) * TILE + w * TOK);
         for (int tile = tiles - 1; tile >= until; --tile) {
             const int t0 = tile * TILE + w * TOK, tokens = min(max(len - t0, 0), TOK);
-            const float left = forwards ? p.ckpt[((ckpt_slot(p, n, bos) + tile) * p.blocks + block) * 256 + e] : 0.f;
+            const float left = forwards ? entered[tile * (p.blocks * 256LL) + e] : 0.f;
             float x[V], z[V], dy[V], v[V], ev[V], gz[V], delta[V], ee[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) { x[i] = rx[i]; z[i] = rz[i]; dy[i] = rdy[i]; v[i] = rdt[i] + bias[i]; }
@@ -266,17 +270,15 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
             }
             at_row -= (long long)TILE * p.DD;
             asm("" : "+s"(at_row));
-            // this block's part of dB and dC: [block of the group][B, C][row][group][S]
             {
-                const long long inner = (long long)p.G * p.S, half = p.rows * inner;
-                float* const to = p.part_bc + 2 * half * (block % p.per_group) + (row0 + t0) * inner + (long long)L.group * p.S;
+                float* const part = part0 + (row0 + t0) * inner;
                 constexpr int PIECES = TOK * LPC < 64 ? 1 : TOK * LPC / 64;
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {
                     const int piece = i * 64 + l, t = piece / LPC, s = piece % LPC * 4;
                     if (t < tokens && s < p.S) {
-                        st_states(to + t * inner + s, my.B[piece], p.S - s, VEC);
-                        st_states(to + half + t * inner + s, my.C[piece], p.S - s, VEC);
+                        st_states(part + t * inner + s, my.B[piece], p.S - s, VEC);
+                        st_states(part + half + t * inner + s, my.C[piece], p.S - s, VEC);
                     }
                 }
             }
@@ -327,8 +329,8 @@ template <typename T, int LPC, int W> static void launch_grad_waves(const ScanAr
     else hipLaunchKernelGGL((scan_grad_kernel<T, LPC, TOK, W, false>), grid, block, 0, s, a);
 }
 template <typename T, int LPC> static void launch_grad(const ScanArgs& a, bool vec, hipStream_t s) {
-    static_assert(SS_TILE_MANY == 4 * SS_TOK && SS_TILE_FEW == 8 * SS_TOK, "a tile begins where a state is left");
-    if (a.every == SS_TILE_MANY) launch_grad_waves<T, LPC, 4>(a, vec, s);
+    static_assert(SS_TILE_MANY == 4 * SS_TOK && SS_TILE_FEW == 8 * SS_TOK && SS_TILE_MANY == 1 << 5 && SS_TILE_FEW == 1 << 6, "a tile begins where a state is left");
+    if (a.every_log2 == 5) launch_grad_waves<T, LPC, 4>(a, vec, s);
     else launch_grad_waves<T, LPC, 8>(a, vec, s);
 }
 template <typename T> static hipError_t launch_scan_grad(const ScanArgs& a, const ScanPlan& s, hipStream_t st) {
