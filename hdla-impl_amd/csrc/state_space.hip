@@ -1,6 +1,6 @@
 // The selective state space scan, forward (state_space.cuh has the formulas and how lanes and waves share the work), and its single-token step.
 //
-// What bounds the scan: the vector ALU, busy 88 to 90 % of the time (8192 x 4096 x 16 191 us, 4 x 2048 x 2048 x 16 75).  A state and token cost 11.3 issue slots in all: a
+// What bounds the scan: the vector ALU, busy 88 to 90 % of the time (8192 x 4096 x 16 191 us, 4 x 2048 x 2048 x 16 72, with the states for a backward pass some 90).  A state and token cost 11.3 issue slots in all: a
 // multiplication and an exponential (two slots) for the decay, two for the walk from zero and two for the other; the rest are step sizes, gates, sums over lanes and what
 // brings operands into place.  Against that stand 8 bytes of x, dt, z and y a channel and token of bf16.
 #include "hdla_launch.h"
