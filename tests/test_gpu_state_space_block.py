@@ -252,3 +252,39 @@ def test_a_state_that_a_graph_keeps_is_not_written_over_unnoticed(native, monkey
         near = rn(2, 3, 16)
         short_conv_step(rn(2, 16), near, w, inplace=True)
     torch.cuda.synchronize()
+
+
+def test_offsets_past_32_bits():
+    # 2^31 elements and more, of which the last rows are compared with a call on these alone; a convolution's and a norm's bits do not depend on the rest
+    T, d, tail = 2 ** 22 + 77, 512, 300
+    g = torch.Generator(device=DEV).manual_seed(12)
+    rn = lambda *s: torch.randn(*s, generator=g, device=DEV, dtype=torch.bfloat16)
+    x = rn(1, T, d)
+    assert x.numel() > 2 ** 31
+    end = lambda t: t[:, T - tail:].contiguous()
+    w, b = rn(d, 4), rn(d)
+    xe = x.detach().requires_grad_()
+    y, _ = short_conv(xe, w, b, activation="silu")
+    dx, = torch.autograd.grad(y, xe, x)
+    ye, _ = short_conv(end(x), w, b, activation="silu", initial_state=x[:, T - tail - 3:T - tail].contiguous())
+    assert torch.equal(y[:, T - tail:].detach(), ye)
+    xs = x[:, T - tail - 3:].contiguous().requires_grad_()
+    ds, = torch.autograd.grad(short_conv(xs, w, b, activation="silu")[0], xs, x[:, T - tail - 3:].contiguous())
+    assert torch.equal(dx[:, T - tail:], ds[:, 3:])
+    del y, dx, ds
+
+    n, r = block_norm(x, x, w[:, 0].contiguous(), post_norm=True, gate=x)
+    ne, re = block_norm(end(x), end(x), w[:, 0].contiguous(), post_norm=True, gate=end(x))
+    assert torch.equal(n[:, T - tail:], ne) and torch.equal(r[:, T - tail:], re)
+    del n, r
+
+    # half a step of each side's rounding to bf16, and of sums whose terms' absolute values stay below 2^10 some 2^7 roundings of 2^-24
+    close = lambda a, b: ((a.double() - b.double()).abs() <= 2.0 ** -8 * (a.double().abs() + b.double().abs()) + 2.0 ** -7).all()
+    A, BC = -0.5 - torch.rand(d, 4, generator=g, device=DEV), rn(1, T, 4)
+    grads = lambda x, BC, h0: torch.autograd.grad(state_space_scan(x, x.detach(), A, BC, BC, dt_softplus=True, initial_state=h0)[0], x, x.detach())[0]
+    _, h = state_space_scan(x[:, :T - tail], x[:, :T - tail], A, BC[:, :T - tail], BC[:, :T - tail], dt_softplus=True, output_final_state=True)
+    y, hT = state_space_scan(x, x, A, BC, BC, dt_softplus=True, output_final_state=True)
+    ye, he = state_space_scan(end(x), end(x), A, end(BC), end(BC), dt_softplus=True, initial_state=h, output_final_state=True)
+    assert close(y[:, T - tail:], ye) and close(hT, he)
+    del y
+    assert close(grads(xe, BC, None)[:, T - tail:], grads(end(x).requires_grad_(), end(BC), h))
