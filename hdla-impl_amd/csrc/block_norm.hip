@@ -252,7 +252,7 @@ __global__ __launch_bounds__(RowShare<WAVES>::THREADS) void block_norm_grad_kern
             for (int j = 0; j < N; ++j) acc[k][i][j] = 0.f;
     }
     for (int turn = turns; turn > 0; --turn, at.row += at.step) {
-        const int E = at.row < p.rows ? p.E : 0;
+        const int E = at.row < p.rows ? p.E : 0;          // (places behind the last row: zeros, and no roots of eps, which may be zero, so that they add nothing to the sums)
         // xhat; r; dy, then the gradient of xhat; the gradient of r; act(gate) and its derivative
         float x[NV][N], r[NV][N], m[NV][N], t[NV][N], a[NV][N], da[NV][N];
         float inv = 1.f, s1[1] = {0.f};
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(RowShare<WAVES>::THREADS) void block_norm_grad_kern
         if (turn > 1) request(at.row + at.step);
         if (p.post_norm) {
             sum1(s1);
-            inv = 1.f / sqrtf(__builtin_fmaf(s1[0], p.inv_e, p.eps));
+            inv = E ? 1.f / sqrtf(__builtin_fmaf(s1[0], p.inv_e, p.eps)) : 0.f;
         }
         float s2[2] = {0.f, 0.f};
 #pragma unroll
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(RowShare<WAVES>::THREADS) void block_norm_grad_kern
                 s2[1] = __builtin_fmaf(m[i][j] * w[i][j], r[i][j], s2[1]);
             }
         sum2(s2);
-        const float ir = 1.f / sqrtf(__builtin_fmaf(s2[0], p.inv_e, p.eps)), along = s2[1] * ir * p.inv_e;
+        const float ir = E ? 1.f / sqrtf(__builtin_fmaf(s2[0], p.inv_e, p.eps)) : 0.f, along = s2[1] * ir * p.inv_e;
         s1[0] = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
