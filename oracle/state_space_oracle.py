@@ -117,12 +117,17 @@ def scan_magnitudes(x, dt, A, B, C, D=None, z=None, bias=None, softplus=False, h
     return m, 2 * longest * step + T * nb + d + 64
 
 
+def gate_sigmoid(g):
+    """The sigmoid with the derivative s sigmoid(-g): torch.sigmoid's s (1 - s) is zero above 37 in float64."""
+    return torch.exp(torch.nn.functional.logsigmoid(g))
+
+
 def block_norm(x, residual=None, weight=None, post_norm=False, post_weight=None, gate=None, act="sigmoid", scale=1.0, eps=1e-5):
     rms = lambda t: torch.sqrt(t.pow(2).mean(-1, keepdim=True) + eps)
     p = x / rms(x) if post_norm or post_weight is not None else x
     p = p if post_weight is None else p * post_weight
     if gate is not None:
-        p = p * (torch.sigmoid(gate) if act == "sigmoid" else silu(gate) if act == "silu" else gate)
+        p = p * (gate_sigmoid(gate) if act == "sigmoid" else silu(gate) if act == "silu" else gate)
     r = scale * p if residual is None else residual + scale * p
     y = r / rms(r)
     return (y if weight is None else y * weight), r
@@ -145,7 +150,7 @@ def block_norm_magnitudes(x, residual=None, weight=None, post_norm=False, post_w
         a, da = torch.ones_like(x), torch.zeros_like(x)
     else:
         s = torch.sigmoid(gate)
-        a, da = {"sigmoid": (s, s * (1 - s)), "silu": ((gate * s).abs(), (s * (1 + gate * (1 - s))).abs() + 0.1)}.get(act, (gate.abs(), torch.ones_like(x)))
+        a, da = {"sigmoid": (s, s * torch.sigmoid(-gate)), "silu": ((gate * s).abs(), (s * (1 + gate * (1 - s))).abs() + 0.1)}.get(act, (gate.abs(), torch.ones_like(x)))
     u = p * a
     r = sc * u + (0 if residual is None else residual.abs())
     _, true = block_norm(x, residual, weight, post_norm, post_weight, gate, act, scale, eps)
