@@ -161,11 +161,13 @@ template <typename T, int V, bool VEC> __device__ __forceinline__ void st_values
 __device__ __forceinline__ float ld_param(const void* p, int f32, long long i) {
     return f32 ? static_cast<const float*>(p)[i] : ld_elem(static_cast<const bf16*>(p) + i);
 }
-// A decay as it stands in the exponent, in base 2.  The lowest finite number for minus infinity, whose product with the step size zero of a place without a token is no number.
-__device__ __forceinline__ float ld_decay(const void* p, int f32, long long i) {
-    const float a = ld_param(p, f32, i) * LOG2E;
+// A decay as it stands in the exponent, in base 2.  The lowest finite number for minus infinity, whose product with a step size of zero is no number: so a place without a token,
+// and a token that is passed over, leave a state as it is.
+__device__ __forceinline__ float decay_exponent(float A) {
+    const float a = A * LOG2E;
     return a < -3.402823466e38f ? -3.402823466e38f : a;
 }
+__device__ __forceinline__ float ld_decay(const void* p, int f32, long long i) { return decay_exponent(ld_param(p, f32, i)); }
 // four states of a channel, the first `n` of which there are
 __device__ __forceinline__ f32x4 ld_states(const float* p, int n, bool whole) {
     if (whole) return *reinterpret_cast<const f32x4*>(p);

@@ -204,11 +204,13 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs p, int lpc_log2
         else z[i].clear();
     }
     const long long a0 = (long long)d * p.S + 4 * q;
-    if (VEC && p.A_f32 && left) A = *reinterpret_cast<const f32x4*>(static_cast<const float*>(p.A) + a0) * LOG2E;
+    if (VEC && p.A_f32 && left) A = *reinterpret_cast<const f32x4*>(static_cast<const float*>(p.A) + a0);
     else
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (j < left) A[j] = ld_param(p.A, p.A_f32, a0 + j) * LOG2E;
+            if (j < left) A[j] = ld_param(p.A, p.A_f32, a0 + j);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) A[j] = decay_exponent(A[j]);
     const float bias = p.bias ? ld_param(p.bias, p.bias_f32, d) : 0.f, D = p.D ? ld_param(p.D, p.D_f32, d) : 0.f;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {

@@ -366,7 +366,8 @@ def state_space_scan(
         delta_t = softplus(dt_t + dt_bias)     (``dt_softplus``; else without it)
         h_t = exp(delta_t A) h_{t-1} + delta_t x_t B_t,     y_t = (C_t . h_t + D x_t) silu(z_t)
 
-    ``A`` is what stands in the exponent: negative where states decay; one that lets them grow must not do so by more than 2^127 over a call.  Returns ``(y [B, T, D] in x's dtype, final_state [N, D, S] fp32 or None)``;
+    ``A`` is what stands in the exponent: negative where states decay; one that lets them grow must not do so by more than 2^127 over a call;
+    minus infinity forgets a state at every step size but zero, which leaves it as it is.  Returns ``(y [B, T, D] in x's dtype, final_state [N, D, S] fp32 or None)``;
     ``cu_seqlens`` packs N sequences into a batch of one.  x, dt, B, C and z of different types are computed in fp32."""
     out = _lib.native().state_space_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state, cu_seqlens)
     if out is not None:
