@@ -76,7 +76,7 @@ def block_norm(
     ``y = r / rms(r) * weight``, with ``rms(v) = sqrt(mean(v^2) + eps)`` over the last dimension.  Returns ``(y in x's dtype, r in residual's)``.
 
     ``gate_act``: "sigmoid", "silu" or None (the gate multiplies as it is).  ``residual_scale``: a number, or a tensor [E] (learned).  The stream may be fp32 beside
-    bf16 blocks.  E is at most 4096.  ``y`` is formed from the sum before that is rounded to the stream's type."""
+    bf16 blocks; other mixtures of types, and fp16, are computed in fp32.  E is at most 4096.  ``y`` is formed from the sum before that is rounded to the stream's type."""
     out = _lib.native().block_norm(x, residual, weight, post_norm, post_weight, gate, gate_act, residual_scale, eps)
     if out is not None:
         return out
@@ -99,9 +99,9 @@ def block_norm(
     for t in (x, residual):
         if t is not None and t.dtype not in _NATIVE + (torch.float16,):
             raise TypeError(f"unsupported dtype {t.dtype}")
-    if out_dtype == torch.float16 or stream == torch.float16 or (out_dtype == torch.float32 and stream != torch.float32):
-        x, residual = x.float(), None if residual is None else residual.float()
-    gate = None if gate is None else gate.to(x.dtype)
+    # fp32, which holds what each of them says, but where the kernels take the types as they are: one of all, or an fp32 stream beside bf16
+    if out_dtype == torch.float16 or stream == torch.float16 or (out_dtype == torch.float32 and stream != torch.float32) or (gate is not None and gate.dtype != out_dtype):
+        x, residual, gate = (None if t is None else t.float() for t in (x, residual, gate))
     weight, post_weight, scale = (None if t is None else param(t).contiguous() for t in (weight, post_weight, scale))
     y, r = BlockNormFunction.apply(whole(x), whole(residual), weight, post_weight, whole(gate), scale, _ACTS[gate_act], bool(post_norm) or post_weight is not None,
                                    1.0 if scale is not None else float(residual_scale), float(eps))
