@@ -92,6 +92,11 @@ def _conv_dims(x, weight, bias, silu, n, cu):
                              step(x, 0), step(x, 1) if x.dim() == 3 else 0, None if cu is None else cu.data_ptr())
 
 
+def _own(dtype, state):
+    """What is computed in: x's type if the state has it too, else fp32, which holds what each of them says."""
+    return dtype if dtype in _NATIVE and (state is None or state.dtype == dtype) else torch.float32
+
+
 def _conv_args(x, weight, bias, activation):
     """Checks of what both calls share."""
     if weight.dim() != 2 or weight.shape[0] != x.shape[-1]:
@@ -159,7 +164,8 @@ def short_conv(
     (``activation="silu"``) ``p_t sigmoid(p_t)``.  W is 2, 3 or 4.
 
     ``initial_state`` holds the W - 1 inputs before each sequence (zeros without it), the returned ``final_state`` its last W - 1, both oldest first;
-    ``cu_seqlens`` packs N sequences into a batch of one.  Returns ``(y, final_state)``, both in x's dtype."""
+    ``cu_seqlens`` packs N sequences into a batch of one.  Returns ``(y, final_state)``, both in x's dtype; an ``initial_state`` of another dtype is
+    computed with in fp32."""
     out = _lib.native().short_conv(x, weight, bias, activation, initial_state, output_final_state, cu_seqlens)
     if out is not None:
         return out
@@ -170,10 +176,9 @@ def short_conv(
     _within_reach(x, n)
     on_one_gpu(x, weight, bias, initial_state)
     out_dtype = x.dtype
-    if out_dtype == torch.float16:
-        x = x.float()
-    elif out_dtype not in _NATIVE:
+    if out_dtype not in _NATIVE + (torch.float16,):
         raise TypeError(f"unsupported dtype {out_dtype}")
+    x = x.to(_own(out_dtype, initial_state))
     state = None if initial_state is None else whole(initial_state.to(x.dtype))
     w, b = param(weight).contiguous(), None if bias is None else param(bias).contiguous()
     y, last = ShortConvFunction.apply(rows(x), w, b, state, silu, bool(output_final_state), n, cu)
@@ -226,8 +231,8 @@ def short_conv_step(
     activation: Optional[str] = None,
     inplace: bool = False,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """``short_conv`` for one token of each sequence: returns ``(y [B, D], new_state)``.  ``inplace=True`` writes the new state where ``state`` is, as
-    a loop of decode steps or a captured graph wants it.  No gradients."""
+    """``short_conv`` for one token of each sequence: returns ``(y [B, D], new_state)``, both in x's dtype.  ``inplace=True`` writes the new state where
+    ``state`` is, as a loop of decode steps or a captured graph wants it: of x's dtype, or fp32.  No gradients."""
     out = _lib.native().short_conv_step(x, state, weight, bias, activation, inplace)
     if out is not None:
         return out
@@ -241,7 +246,7 @@ def short_conv_step(
     out_dtype = x.dtype
     if out_dtype not in _NATIVE + (torch.float16,):
         raise TypeError(f"unsupported dtype {out_dtype}")
-    own = torch.float32 if out_dtype == torch.float16 else out_dtype
+    own = _own(out_dtype, state)
     to = _new_state(state, inplace, own)
 
     def call(x, state, weight, bias):
