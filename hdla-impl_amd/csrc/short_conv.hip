@@ -450,7 +450,8 @@ static int conv_check(const hdla_conv_dims* d) {
     if (!d) return HDLA_ERR_NULL;
     for (int t : {d->dtype, d->weight_dtype, d->bias_dtype})
         if (t != HDLA_BF16 && t != HDLA_FP32) return HDLA_ERR_DTYPE;
-    if (d->B < 1 || d->T < 0 || d->D < 1 || d->N < 1 || d->W < 2 || d->W > 4 || d->T > (1 << 30) || d->D > (1 << 24)) return HDLA_ERR_SHAPE;
+    const bool none = d->B == 0 && d->N == 0;             // no sequences
+    if ((!none && (d->B < 1 || d->N < 1)) || d->T < 0 || d->D < 1 || d->W < 2 || d->W > 4 || d->T > (1 << 30) || d->D > (1 << 24)) return HDLA_ERR_SHAPE;
     if (d->cu_seqlens ? d->B != 1 : d->N != d->B) return HDLA_ERR_SEQ;
     if ((long long)d->B * d->T > 0x7fffffffLL) return HDLA_ERR_SHAPE;
     return HDLA_OK;
@@ -553,6 +554,7 @@ extern "C" int hdla_short_conv_step(const hdla_conv_dims* dims, const void* x, c
     const int rc = conv_check(dims);
     if (rc) return rc;
     if (dims->T != 1 || dims->cu_seqlens) return HDLA_ERR_SHAPE;
+    if (!dims->N) return HDLA_OK;
     if (!x || !weight || !state || !y || !new_state) return HDLA_ERR_NULL;
     for (const void* q : {state, (const void*)y, (const void*)new_state})
         if (!fits(q, 16)) return HDLA_ERR_ALIGN;

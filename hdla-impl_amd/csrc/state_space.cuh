@@ -347,6 +347,7 @@ struct ScanPlan {
 // ones the longest is taken for twice the average) against segments of the length that is best, which have to gain an eighth.
 inline void scan_segments(const hdla_scan_dims* d, ScanPlan& s, float cost) {
     constexpr long long CUS = 256;
+    if (!d->N) return;
     const bool packed = d->cu_seqlens != nullptr;
     const long long average = d->T / (packed ? d->N : 1), longest = packed && d->N > 1 ? std::min<long long>(2 * average, d->T) : d->T;
     const long long wide = scan_workgroups(s.blocks, 1);
@@ -372,7 +373,8 @@ inline int scan_plan(const hdla_scan_dims* d, ScanPlan& s) {
     if (d->dtype != HDLA_BF16 && d->dtype != HDLA_FP32) return HDLA_ERR_DTYPE;
     for (int t : {d->A_dtype, d->D_dtype, d->bias_dtype})
         if (t != HDLA_BF16 && t != HDLA_FP32) return HDLA_ERR_DTYPE;
-    if (d->B < 1 || d->T < 0 || d->D < 1 || d->S < 1 || d->S > 64 || d->G < 1 || d->D % d->G || d->N < 1) return HDLA_ERR_SHAPE;
+    const bool none = d->B == 0 && d->N == 0;             // no sequences
+    if ((!none && (d->B < 1 || d->N < 1)) || d->T < 0 || d->D < 1 || d->S < 1 || d->S > 64 || d->G < 1 || d->D % d->G) return HDLA_ERR_SHAPE;
     if (d->cu_seqlens ? d->B != 1 : d->N != d->B) return HDLA_ERR_SEQ;
     if (d->T > (1 << 30) || d->D > ROW_MOST) return HDLA_ERR_SHAPE;
     for (long long r : {d->x_row, d->dt_row, d->z_row, d->B_row, d->C_row})

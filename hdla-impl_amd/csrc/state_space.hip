@@ -293,6 +293,7 @@ extern "C" int hdla_scan_fwd(const hdla_scan_dims* dims, const void* x, const vo
     if (!A || (s.rows > 0 && (!x || !dt || !B || !C || !y))) return HDLA_ERR_NULL;
     if (!fits(y, 16) || !fits(h0, 16) || !fits(ht, 16)) return HDLA_ERR_ALIGN;
     if (states && (!fits(states, 16) || states_bytes < (size_t)s.ckpt * s.blocks * 1024)) return HDLA_ERR_WORKSPACE;
+    if (!s.units) return HDLA_OK;
     scan_segments(dims, s, SEGMENT_COST_FORWARD);
     if (s.seg && (!workspace || !fits(workspace, 16) || workspace_bytes < ends_bytes(s))) return HDLA_ERR_WORKSPACE;
     ScanArgs a = scan_args(dims, s, x, dt, A, B, C, D, z, dt_bias);
@@ -318,6 +319,7 @@ extern "C" int hdla_scan_step(const hdla_scan_dims* dims, const void* x, const v
     const int rc = scan_plan(dims, s);
     if (rc) return rc;
     if (dims->T != 1 || dims->cu_seqlens) return HDLA_ERR_SHAPE;
+    if (!dims->N) return HDLA_OK;
     if (!x || !dt || !A || !B || !C || !y || !state || !new_state) return HDLA_ERR_NULL;
     if (!fits(y, 16) || !fits(state, 16) || !fits(new_state, 16)) return HDLA_ERR_ALIGN;
     ScanArgs a = scan_args(dims, s, x, dt, A, B, C, D, z, dt_bias);

@@ -321,7 +321,7 @@ static int grad_slots(const ScanPlan& s) {
 // partial sums of dB and dC, [blocks of a group][2][rows][G][S], and behind them those of dA, dD and d bias, [slots][D S + 2 D], and segments' ends
 static size_t bc_bytes(const hdla_scan_dims* d, const ScanPlan& s) { return ((size_t)s.per_group * 2 * s.rows * d->G * d->S * 4 + 15) / 16 * 16; }
 static size_t own_bytes(const hdla_scan_dims* d, int slots) { return ((size_t)slots * d->D * (d->S + 2) * 4 + 15) / 16 * 16; }
-static size_t grad_bytes(const hdla_scan_dims* d, const ScanPlan& s, int slots) { return bc_bytes(d, s) + own_bytes(d, slots) + ends_bytes(s); }
+static size_t grad_bytes(const hdla_scan_dims* d, const ScanPlan& s, int slots) { return std::max<size_t>(bc_bytes(d, s) + own_bytes(d, slots) + ends_bytes(s), 16); }
 template <typename T, int LPC, int W> static void launch_grad_waves(const ScanArgs& a, bool vec, hipStream_t s) {
     constexpr int TOK = SS_TOK;
     const dim3 grid((unsigned)scan_workgroups(a.blocks, a.slots)), block(64 * W);
@@ -388,7 +388,7 @@ extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const vo
         const hipError_t e = dims->dtype == HDLA_BF16 ? launch_scan_ends<bf16>(a, s, true, st) : launch_scan_ends<float>(a, s, true, st);
         if (e != hipSuccess) return (int)e;
     }
-    hipError_t e = dims->dtype == HDLA_BF16 ? launch_scan_grad<bf16>(a, s, st) : launch_scan_grad<float>(a, s, st);
+    hipError_t e = !s.units ? hipSuccess : dims->dtype == HDLA_BF16 ? launch_scan_grad<bf16>(a, s, st) : launch_scan_grad<float>(a, s, st);
     if (e != hipSuccess) return (int)e;
     ColumnSums c{};
     const long long inner = (long long)dims->G * dims->S;

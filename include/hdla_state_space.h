@@ -1,7 +1,8 @@
 /* libhdla_hip.so -- C ABI of the operators of a state space block: the short causal convolution, the selective state space scan, the norms around a block.
  *
  * Conventions are those of hdla_hip.h (device pointers, streams, workspaces, return codes), but that x, dt, z, B and C of the scan and x of the convolution may
- * lie at any address and with strides of their own.  dtype codes: HDLA_BF16, HDLA_FP32. */
+ * lie at any address and with strides of their own.  dtype codes: HDLA_BF16, HDLA_FP32.  A batch of no sequences (B = N = 0) leaves zeros in the gradients of
+ * parameters and touches nothing else. */
 #ifndef HDLA_STATE_SPACE_H
 #define HDLA_STATE_SPACE_H
 
