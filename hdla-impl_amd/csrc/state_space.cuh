@@ -55,6 +55,7 @@ struct ScanArgs {
     float *part_bc, *part_own, *dh0;
     long long rows;
     int slots;                        // units (sequences, or segments of them) at a time
+    int first, take;                  // blocks of each group that a pass has, from the first on
     // segments: 0, or how many tokens one has; `units` of them, and for each [blocks][256] what it leaves if nothing enters, and [blocks][256] its decays
     int seg, units;
     float* ends;
@@ -339,18 +340,19 @@ inline int lanes_of(int S) { return S <= 8 ? 2 : S <= 16 ? 4 : S <= 32 ? 8 : 16;
 
 // What both passes and the workspace sizes go by
 struct ScanPlan {
-    int lpc, per_group, blocks, slots, seg, every;
+    int lpc, per_group, blocks, slots, seg, every, take, passes;
     bool vec;
     long long rows, ckpt, units;
 };
 // Segments fill the device where there are few (sequence, channel block) pairs, at `cost` times the work.  In tokens that a compute unit walks: whole sequences (of packed
-// ones the longest is taken for twice the average) against segments of the length that is best, which have to gain an eighth.
-inline void scan_segments(const hdla_scan_dims* d, ScanPlan& s, float cost) {
+// ones the longest is taken for twice the average) against segments of the length that is best, which have to gain an eighth.  `at_once`: channel blocks that are worked on
+// together.
+inline void scan_segments(const hdla_scan_dims* d, ScanPlan& s, float cost, int at_once) {
     constexpr long long CUS = 256;
     if (!d->N) return;
     const bool packed = d->cu_seqlens != nullptr;
     const long long average = d->T / (packed ? d->N : 1), longest = packed && d->N > 1 ? std::min<long long>(2 * average, d->T) : d->T;
-    const long long wide = scan_workgroups(s.blocks, 1);
+    const long long wide = scan_workgroups(at_once, 1);
     auto rounds = [](long long wgs) { return (wgs + CUS - 1) / CUS; };
     const long long all = wide * d->N;
     float best = 0.875f * (float)std::max<long long>(longest, rounds(all) * average);

@@ -282,7 +282,7 @@ extern "C" int hdla_state_space_version(void) { return HDLA_STATE_SPACE_VERSION;
 extern "C" size_t hdla_scan_fwd_workspace_bytes(const hdla_scan_dims* dims) {
     ScanPlan s;
     if (scan_plan(dims, s)) return 0;
-    scan_segments(dims, s, SEGMENT_COST_FORWARD);
+    scan_segments(dims, s, SEGMENT_COST_FORWARD, s.blocks);
     return ends_bytes(s);
 }
 extern "C" int hdla_scan_fwd(const hdla_scan_dims* dims, const void* x, const void* dt, const void* A, const void* B, const void* C, const void* D, const void* z,
@@ -294,7 +294,7 @@ extern "C" int hdla_scan_fwd(const hdla_scan_dims* dims, const void* x, const vo
     if (!fits(y, 16) || !fits(h0, 16) || !fits(ht, 16)) return HDLA_ERR_ALIGN;
     if (states && (!fits(states, 16) || states_bytes < (size_t)s.ckpt * s.blocks * 1024)) return HDLA_ERR_WORKSPACE;
     if (!s.units) return HDLA_OK;
-    scan_segments(dims, s, SEGMENT_COST_FORWARD);
+    scan_segments(dims, s, SEGMENT_COST_FORWARD, s.blocks);
     if (s.seg && (!workspace || !fits(workspace, 16) || workspace_bytes < ends_bytes(s))) return HDLA_ERR_WORKSPACE;
     ScanArgs a = scan_args(dims, s, x, dt, A, B, C, D, z, dt_bias);
     a.h0 = h0; a.ht = ht; a.y = y; a.ckpt = static_cast<float*>(states); a.ends = static_cast<float*>(workspace);

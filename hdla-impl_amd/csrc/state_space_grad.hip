@@ -36,7 +36,8 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
     __shared__ Meet meet;
 
     int slot, block;
-    if (!scan_work(blockIdx.x, p.blocks, slot, block)) return;
+    if (!scan_work(blockIdx.x, p.take * p.G, slot, block)) return;
+    if (p.take < p.per_group) block = block / p.take * p.per_group + p.first + block % p.take;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id(), tid = threadIdx.x;
     const Lane L(p, block);
     Mine& my = mine[w];
@@ -92,9 +93,9 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
             cx.next(); cdt.next(); cz.next(); cdy.next(); cB.next(); cC.next();
         };
         const float* const entered = ckpt_of(p, n, bos, block);
-        // this block's part of dB and dC: [block of the group][B, C][row][group][S]
+        // this block's part of dB and dC: [block of the group in this pass][B, C][row][group][S]
         const long long inner = (long long)p.G * p.S, half = p.rows * inner;
-        float* const part0 = p.part_bc + 2 * half * (block % p.per_group) + (long long)L.group * p.S;
+        float* const part0 = p.part_bc + 2 * half * (block % p.per_group - p.first) + (long long)L.group * p.S;
         request((tiles - 1) * TILE + w * TOK);
         for (int tile = tiles - 1; tile >= until; --tile) {
             const int t0 = tile * TILE + w * TOK, tokens = min(max(len - t0, 0), TOK);
@@ -271,14 +272,14 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
             at_row -= (long long)TILE * p.DD;
             asm("" : "+s"(at_row));
             {
-                float* const part = part0 + (row0 + t0) * inner;
+                float* const to = part0 + (row0 + t0) * inner;
                 constexpr int PIECES = TOK * LPC < 64 ? 1 : TOK * LPC / 64;
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {
                     const int piece = i * 64 + l, t = piece / LPC, s = piece % LPC * 4;
                     if (t < tokens && s < p.S) {
-                        st_states(part + t * inner + s, my.B[piece], p.S - s, VEC);
-                        st_states(part + half + t * inner + s, my.C[piece], p.S - s, VEC);
+                        st_states(to + t * inner + s, my.B[piece], p.S - s, VEC);
+                        st_states(to + half + t * inner + s, my.C[piece], p.S - s, VEC);
                     }
                 }
             }
@@ -313,18 +314,35 @@ __global__ __launch_bounds__(64 * W) void scan_grad_kernel(ScanArgs p) {
     }
 }
 
-// Workgroups walk sequences, or segments, in turns so that their partial sums of dA, dD and d bias stay few: as many as fill the device a few times
-static int grad_slots(const ScanPlan& s) {
-    const long long most = std::max(1LL, 2048LL / s.blocks);
-    return (int)std::min<long long>(s.units, most);
+// Partial sums of dB and dC are a fp32 copy of both for every block of 64 / lanes channels: with more channels and states they outgrow everything else (8192 channels with 64 states: 64
+// times x in bf16).  So a pass takes as many blocks of a group as fit into PARTS_MOST, and the next one goes on with their sums, which lie in front of its own parts: the same additions in the
+// same order as in one pass.  ms a training step and GB of parts, in one pass / so, with 4096 channels and 64 states in bf16: 4 x 2048 tokens 3.91 and 4.3 / 3.95 and 2.2, 1 x 32768 (whose
+// passes are cut into segments) 16.1 and 17.2 / 17.7 and 2.2.
+constexpr size_t PARTS_MOST = (size_t)2 << 30;
+static size_t part_floats(const hdla_scan_dims* d, const ScanPlan& s) { return 2 * (size_t)s.rows * d->G * d->S; }
+static void grad_plan(const hdla_scan_dims* d, ScanPlan& s) {
+    const size_t one = part_floats(d, s) * 4;
+    s.take = s.per_group;
+    s.passes = 1;
+    if (s.per_group * one > PARTS_MOST) {
+        // (as many as are whole rounds of two workgroups a compute unit, where a round fits)
+        const long long most = std::max<size_t>(PARTS_MOST / one, 1), full = std::max(1LL, 512 / ((long long)d->G * d->N)), round = most < full ? 1 : full;
+        const long long rounds = (s.per_group + round - 1) / round, passes = (rounds + most / round - 1) / (most / round);
+        s.take = (int)((rounds + passes - 1) / passes * round);
+        s.passes = (s.per_group + s.take - 1) / s.take;
+    }
+    scan_segments(d, s, SEGMENT_COST_BACKWARD, s.take * d->G);
+    // Workgroups walk sequences, or segments, in turns so that their partial sums of dA, dD and d bias stay few: as many as fill the device a few times
+    s.slots = (int)std::min<long long>(s.units, std::max(1LL, 2048LL / (s.take * d->G)));
 }
-// partial sums of dB and dC, [blocks of a group][2][rows][G][S], and behind them those of dA, dD and d bias, [slots][D S + 2 D], and segments' ends
-static size_t bc_bytes(const hdla_scan_dims* d, const ScanPlan& s) { return ((size_t)s.per_group * 2 * s.rows * d->G * d->S * 4 + 15) / 16 * 16; }
-static size_t own_bytes(const hdla_scan_dims* d, int slots) { return ((size_t)slots * d->D * (d->S + 2) * 4 + 15) / 16 * 16; }
-static size_t grad_bytes(const hdla_scan_dims* d, const ScanPlan& s, int slots) { return std::max<size_t>(bc_bytes(d, s) + own_bytes(d, slots) + ends_bytes(s), 16); }
+// partial sums of dB and dC, [sum of earlier passes, where there are several; blocks of a group in a pass][2][rows][G][S], and behind them those of dA, dD and d bias, [slots][D S + 2 D],
+// and segments' ends
+static size_t bc_bytes(const hdla_scan_dims* d, const ScanPlan& s) { return ((s.take + (s.passes > 1)) * part_floats(d, s) * 4 + 15) / 16 * 16; }
+static size_t own_bytes(const hdla_scan_dims* d, const ScanPlan& s) { return ((size_t)s.slots * d->D * (d->S + 2) * 4 + 15) / 16 * 16; }
+static size_t grad_bytes(const hdla_scan_dims* d, const ScanPlan& s) { return std::max<size_t>(bc_bytes(d, s) + own_bytes(d, s) + ends_bytes(s), 16); }
 template <typename T, int LPC, int W> static void launch_grad_waves(const ScanArgs& a, bool vec, hipStream_t s) {
     constexpr int TOK = SS_TOK;
-    const dim3 grid((unsigned)scan_workgroups(a.blocks, a.slots)), block(64 * W);
+    const dim3 grid((unsigned)scan_workgroups(a.take * a.G, a.slots)), block(64 * W);
     if (vec) hipLaunchKernelGGL((scan_grad_kernel<T, LPC, TOK, W, true>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((scan_grad_kernel<T, LPC, TOK, W, false>), grid, block, 0, s, a);
 }
@@ -351,8 +369,8 @@ using namespace hdla;
 extern "C" size_t hdla_scan_workspace_bytes(const hdla_scan_dims* dims) {
     ScanPlan s;
     if (scan_plan(dims, s)) return 0;
-    scan_segments(dims, s, SEGMENT_COST_BACKWARD);
-    return grad_bytes(dims, s, grad_slots(s));
+    grad_plan(dims, s);
+    return grad_bytes(dims, s);
 }
 extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const void* dt, const void* A, const void* B, const void* C, const void* D, const void* z,
                              const void* dt_bias, const void* dy, const float* dht, const void* states, size_t states_bytes, void* dx, void* ddt, void* dA, void* dB,
@@ -364,17 +382,17 @@ extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const vo
     if (s.rows > 0 && (!x || !dt || !B || !C || !dy || !dx || !ddt || !dB || !dC || !states || (z && !dz))) return HDLA_ERR_NULL;
     for (const void* q : {dy, (const void*)dht, states, (const void*)dx, (const void*)ddt, (const void*)dB, (const void*)dC, (const void*)dz, (const void*)dh0})
         if (!fits(q, 16)) return HDLA_ERR_ALIGN;
-    scan_segments(dims, s, SEGMENT_COST_BACKWARD);
-    s.slots = grad_slots(s);
-    if (!workspace || !fits(workspace, 16) || workspace_bytes < grad_bytes(dims, s, s.slots)) return HDLA_ERR_WORKSPACE;
+    grad_plan(dims, s);
+    if (!workspace || !fits(workspace, 16) || workspace_bytes < grad_bytes(dims, s)) return HDLA_ERR_WORKSPACE;
     if (s.rows > 0 && states_bytes < (size_t)s.ckpt * s.blocks * 1024) return HDLA_ERR_WORKSPACE;
     ScanArgs a = scan_args(dims, s, x, dt, A, B, C, D, z, dt_bias);
     a.dy = dy; a.dht = dht; a.ckpt = static_cast<float*>(const_cast<void*>(states));
     a.dx = dx; a.ddt = ddt; a.dz = dz; a.dh0 = dh0;
     char* const base = static_cast<char*>(workspace);
-    a.part_bc = reinterpret_cast<float*>(base);
+    float* const sums = reinterpret_cast<float*>(base);   // of earlier passes, where there are several
+    a.part_bc = sums + (s.passes > 1 ? part_floats(dims, s) : 0);
     a.part_own = reinterpret_cast<float*>(base + bc_bytes(dims, s));
-    a.ends = reinterpret_cast<float*>(base + bc_bytes(dims, s) + own_bytes(dims, s.slots));
+    a.ends = reinterpret_cast<float*>(base + bc_bytes(dims, s) + own_bytes(dims, s));
     s.vec = scan_vec(dims, s, a);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const int es = dims->dtype == HDLA_BF16 ? 2 : 4;
@@ -388,19 +406,29 @@ extern "C" int hdla_scan_bwd(const hdla_scan_dims* dims, const void* x, const vo
         const hipError_t e = dims->dtype == HDLA_BF16 ? launch_scan_ends<bf16>(a, s, true, st) : launch_scan_ends<float>(a, s, true, st);
         if (e != hipSuccess) return (int)e;
     }
-    hipError_t e = !s.units ? hipSuccess : dims->dtype == HDLA_BF16 ? launch_scan_grad<bf16>(a, s, st) : launch_scan_grad<float>(a, s, st);
-    if (e != hipSuccess) return (int)e;
-    ColumnSums c{};
-    const long long inner = (long long)dims->G * dims->S;
-    c.part = a.part_bc; c.rows = s.per_group;
-    c.cu = a.cu; c.N = a.N; c.T = a.T; c.per_token = inner; c.tokens_end = 2 * s.rows * inner;
-    c.add(dB, es == 4, s.rows * inner);
-    c.add(dC, es == 4, s.rows * inner);
     ColumnSums k{};
     k.part = a.part_own; k.rows = s.slots;
     k.add(dA, a.A_f32, (long long)dims->D * dims->S);
     k.add(D ? dD : nullptr, a.D_f32, dims->D);
     k.add(dt_bias ? ddt_bias : nullptr, a.bias_f32, dims->D);
-    e = launch_column_sums(c, st, k);
-    return e == hipSuccess ? HDLA_OK : (int)e;
+    const long long inner = (long long)dims->G * dims->S;
+    for (int pass = 0; pass < s.passes; ++pass) {
+        a.first = pass * s.take;
+        a.take = std::min(s.take, s.per_group - a.first);
+        hipError_t e = !s.units ? hipSuccess : dims->dtype == HDLA_BF16 ? launch_scan_grad<bf16>(a, s, st) : launch_scan_grad<float>(a, s, st);
+        if (e != hipSuccess) return (int)e;
+        const bool last = pass + 1 == s.passes;
+        ColumnSums c{};
+        c.part = pass ? sums : a.part_bc; c.rows = a.take + (pass > 0);
+        c.cu = a.cu; c.N = a.N; c.T = a.T; c.per_token = inner; c.tokens_end = 2 * s.rows * inner;
+        if (last) {
+            c.add(dB, es == 4, s.rows * inner);
+            c.add(dC, es == 4, s.rows * inner);
+        } else {
+            c.add(sums, true, 2 * s.rows * inner);        // (a thread writes where it has read)
+        }
+        e = launch_column_sums(c, st, last ? k : ColumnSums{});
+        if (e != hipSuccess) return (int)e;
+    }
+    return HDLA_OK;
 }
