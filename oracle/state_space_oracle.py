@@ -117,6 +117,127 @@ def scan_magnitudes(x, dt, A, B, C, D=None, z=None, bias=None, softplus=False, h
     return m, 2 * longest * step + T * nb + d + 64
 
 
+def scan_bounds(x, dt, A, B, C, D=None, z=None, bias=None, softplus=False, h0=None, cu=None, dy=None, dht=None):
+    """How far each output and gradient of the scan may be off in 32 bits, element by element: errors go through the recurrences as the values do and fade with them.
+
+    u = 2^-24 is half a step.  To first order, with every term by its absolute value:
+      v = dt + bias            u |v|
+      delta = softplus(v)      sigmoid(v) u |v| from v; e = exp(-|v|) is off by 2 |v| + 2 (its exponent's product and constant, the exponential's last place), the rest of log(1 + e) by 8;
+                               the sum by one:  u (sigmoid(v) |v| + 10 delta + 2 |v| log(1 + e))
+      a = exp(delta A)         relative: |A| err(delta) from delta; of the exponent's own 3 u |delta A|, and 8 more where a piece's decay comes from a sum of eight steps; 2 u of the
+                               exponential, 2 u of products of pieces' decays:  rho = |A| err(delta) + u (11 |delta A| + 4); what underflows is off by 2^-125
+      b = delta x B            |x B| err(delta) + 2 u |b|
+      h' = a h + b             a err(h) + (a rho) |h| + err(b) + 3 u |h'|: the walk from zero, the chain over the pieces, the walk from what enters
+      sums over states         four in a lane, at most four exchanges, a product: 10 u
+      sigmoid                  relative: (2 |z| + 2) (1 - s) of its exponential, 4 of sum and reciprocal
+      sums over channels       a lane's exchanges and a block after the other, at least four channels each: u (8 + channels / 4)
+    The gradients g of h go back by the same recurrence.  Sums over all n tokens (dA, dD, d bias) are off by no more than the sum of their terms' bounds and u (n + 16) of the sum of the
+    terms.  Where n is large that is far: roundings do not all fall to one side.  Of errors that are as likely up as down, each within its own bound, the sum's standard deviation is the
+    root of the bounds' squares over 1.7; a rounding that stays in a state for w tokens is w times in the sum, and its tokens' bounds are w times as large.  Four times that root is seven
+    standard deviations, and the smaller of the two is taken."""
+    u, tiny = 2.0 ** -24, 2.0 ** -125
+    nb, T, d = x.shape
+    G, S = B.shape[2], A.shape[1]
+    f = lambda t: None if t is None else t.detach().double()
+    x, dt, A, B, C, D, z, bias, h0, dy, dht = (f(t) for t in (x, dt, A, B, C, D, z, bias, h0, dy, dht))
+    v = dt if bias is None else dt + bias
+    if softplus:
+        s, log = torch.sigmoid(v), torch.log1p(torch.exp(-v.abs()))
+        delta = v.clamp(min=0) + log
+        ed = u * (s * v.abs() + 10 * delta + 2 * v.abs() * log)
+        slope, eslope = s, u * s * (4 + 2 * (3 * v.abs() + 2) * torch.sigmoid(-v))
+    else:
+        delta, ed, slope, eslope = v, u * v.abs(), torch.ones_like(v), torch.zeros_like(v)
+    X, size = x.abs(), delta.abs()
+    if z is None:
+        gate, egate, sl, SL, esl = torch.ones_like(x), torch.zeros_like(x), None, None, None
+    else:
+        s, r = torch.sigmoid(z), torch.sigmoid(-z)
+        es = u * s * ((2 * z.abs() + 2) * r + 4)
+        gate, egate = z.abs() * s, z.abs() * es
+        sl, SL = (s * (1 + z * r)).abs(), s * (1 + z.abs() * r)
+        esl = es * (1 + z * r).abs() + s * z.abs() * es + 3 * u * SL
+    wide = lambda t: t.abs().repeat_interleave(d // G, 0)                    # [G, S] for every channel
+    group = lambda t: t.unflatten(0, (G, d // G)).sum(1)
+    seqs = spans(nb, T, cu)
+    out = {k: torch.zeros_like(t) for k, t in (("y", x), ("x", x), ("dt", x), ("z", x), ("A", A), ("B", B), ("C", C))}
+    zeros = lambda *n: x.new_zeros(*n)
+    out["D"], out["bias"], out["ht"], out["h0"] = zeros(d), zeros(d), zeros(len(seqs), d, S), zeros(len(seqs), d, S)
+    sums = {k: [torch.zeros_like(out[k]) for _ in range(3)] for k in ("A", "D", "bias")}      # over tokens: of bounds, of their squares, of terms
+
+    def token(k, bound, term):
+        for to, t in zip(sums[k], (bound, bound * bound, term)):
+            to += t
+
+    Aa = A.abs()
+
+    def decay(b, t):
+        a = torch.exp(delta[b, t][:, None] * A)
+        rho = Aa * ed[b, t][:, None] + u * (11 * size[b, t][:, None] * Aa + 4)
+        return a, torch.where(a > 0, a * rho, 0 * a) + tiny * ((a > 0) & (a < 2.0 ** -100))
+
+    for n, (b, t0, t1) in enumerate(seqs):
+        h = zeros(d, S) if h0 is None else h0[n].abs()
+        eh = torch.zeros_like(h)
+        hs, ehs = [h], [eh]
+        I, eI = [], []
+        for t in range(t0, t1):
+            a, ea = decay(b, t)
+            Bt, Ct = wide(B[b, t]), wide(C[b, t])
+            add = (size[b, t] * X[b, t])[:, None] * Bt
+            eb = (X[b, t] * ed[b, t])[:, None] * Bt + 2 * u * add
+            eh = a * eh + ea * h + eb
+            h = a * h + add
+            eh = eh + 3 * u * h
+            hs.append(h)
+            ehs.append(eh)
+            inner = (h * Ct).sum(-1) + (0 if D is None else (D * x[b, t]).abs())
+            ei = (eh * Ct).sum(-1) + 10 * u * inner
+            I.append(inner)
+            eI.append(ei)
+            out["y"][b, t] = gate[b, t] * ei + inner * egate[b, t] + 2 * u * inner * gate[b, t]
+        out["ht"][n] = eh
+        if dy is None:
+            continue
+        g = zeros(d, S) if dht is None else dht[n].abs()
+        eg = torch.zeros_like(g)
+        channels = u * (8 + d // G / 4)
+        for t in range(t1 - 1, t0 - 1, -1):
+            i = t - t0
+            a, ea = decay(b, t)
+            Bt, Ct = wide(B[b, t]), wide(C[b, t])
+            Y, Dl, Ed, Xt = dy[b, t].abs(), size[b, t], ed[b, t], X[b, t]
+            e = Y * gate[b, t]
+            ee = Y * egate[b, t] + 2 * u * e
+            g = g + Ct * e[:, None]
+            eg = eg + Ct * ee[:, None] + 3 * u * g
+            out["C"][b, t] = group(hs[i + 1] * ee[:, None] + ehs[i + 1] * e[:, None] + channels * hs[i + 1] * e[:, None])
+            add, eadd = Dl * Xt, Xt * Ed + u * Dl * Xt
+            out["B"][b, t] = group(eg * add[:, None] + g * eadd[:, None] + channels * g * add[:, None])
+            gb = (g * Bt).sum(-1)
+            egb = (eg * Bt).sum(-1) + 10 * u * gb
+            th = a * g * hs[i]
+            eth = a * eg * hs[i] + ea * g * hs[i] + a * g * ehs[i] + 3 * u * th
+            ga = (Aa * th).sum(-1)
+            ega = (Aa * eth).sum(-1) + 14 * u * ga
+            De = 0 if D is None else D.abs() * e
+            out["x"][b, t] = Dl * egb + gb * Ed + (0 if D is None else D.abs() * ee) + 3 * u * (gb * Dl + De)
+            raw, eraw = gb * Xt + ga, Xt * egb + ega + 2 * u * (gb * Xt + ga)
+            out["dt"][b, t] = slope[b, t] * eraw + raw * eslope[b, t] + u * raw * slope[b, t]
+            token("A", Dl[:, None] * eth + th * Ed[:, None], Dl[:, None] * th)
+            token("D", Xt * ee, e * Xt)
+            token("bias", out["dt"][b, t], raw * slope[b, t])
+            if z is not None:
+                out["z"][b, t] = Y * (eI[i] * sl[b, t] + I[i] * esl[b, t] + 2 * u * I[i] * SL[b, t])
+            eg = a * eg + ea * g
+            g = a * g
+        out["h0"][n] = eg + u * g
+    count = nb * T + 16
+    for k, (bound, squares, term) in sums.items():
+        out[k] = torch.minimum(bound + count * u * term, 4 * squares.sqrt() + 4 * count ** 0.5 * u * term)
+    return out
+
+
 def gate_sigmoid(g):
     """The sigmoid with the derivative s sigmoid(-g): torch.sigmoid's s (1 - s) is zero above 37 in float64."""
     return torch.exp(torch.nn.functional.logsigmoid(g))
