@@ -105,7 +105,7 @@ template <typename T, int N> __device__ __forceinline__ void activate(int act, c
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         a[i] = act == ACT_SILU ? g[i] * s[i] : s[i];
-        da[i] = act == ACT_SILU ? s[i] * __builtin_fmaf(g[i], 1.f - s[i], 1.f) : s[i] * (s[i] * fminf(exp_t<T>(-g[i]), 3.402823466e38f));
+        da[i] = act == ACT_SILU ? s[i] * __builtin_fmaf(g[i], 1.f - s[i], 1.f) : s[i] * (s[i] * __builtin_amdgcn_fmed3f(exp_t<T>(-g[i]), 0.f, 3.402823466e38f));
     }
 }
 
