@@ -5,8 +5,9 @@
 // Tiles of 64 or 32 tokens, the last first, each from the state that the forward pass left at its first token.  A wave scans its eight tokens forwards and backwards
 // from zero; both chains over the waves' pieces run at once, four waves each (of four waves: one behind the other); then it walks them again with what enters, states and decays in registers.
 //
-// What bounds it: the vector ALU, busy 76 % of the time (4 x 2048 x 2048 x 16 some 285 us, and 22 for the sums of dB and dC): 30 issue slots a state and token in all, of which two
-// are the exponential, fifteen the other arithmetic of the four walks and four the sums over channels for dB and dC.
+// What bounds it: the vector ALU, busy 76 % of the time (4 x 2048 x 2048 x 16 some 285 us, and 22 for the sums of dB and dC): 30 issue slots a state and token in all (27 instructions; an
+// exponential and a lane swap are two slots), of which two are the exponential, fifteen the other arithmetic of the four walks, six the sums over channels for dB and dC, two the sums over
+// a channel's lanes and five what there is once for a token and channel: step sizes, gates, results, addresses.
 #include "column_sums.cuh"
 #include "hdla_launch.h"
 #include "state_space.cuh"
